@@ -34,7 +34,9 @@ def build(force=False, verbose=True):
 
     objdir = os.path.join(CSRC, "obj")
     os.makedirs(objdir, exist_ok=True)
-    flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"]
+    # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 - some forms of these instructions (the compiler makes them from ordinary
+    # scalar code) have given wrong results on MI355X now and then; the host pass of hipcc warns that it does not know the feature
+    flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     if os.environ.get("DSW_BUILD_DIAG") == "1":      # diagnostics build: enables the DSW_* run-time switches of csrc/
         flags.append("-DDSW_DIAG")
 
