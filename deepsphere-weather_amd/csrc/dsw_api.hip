@@ -252,6 +252,7 @@ const char* dsw_strerror(int code) {
         case DSW_ERR_WORKSPACE: return "workspace too small or null";
         case DSW_ERR_LAUNCH: return "HIP kernel launch failed";
         case DSW_ERR_ALIGN: return "pointer not sufficiently aligned";
+        case DSW_ERR_OVERLAP: return "a written tensor overlaps another tensor of the call";
         default: return "unknown error";
     }
 }

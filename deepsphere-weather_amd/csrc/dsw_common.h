@@ -4,7 +4,7 @@
 #include <hip/hip_ext.h>
 #include <stdint.h>
 
-#define DSW_VERSION 101  // 0.1.1: dsw_hop2_plan carries its own size (struct_bytes)
+#define DSW_VERSION 102  // 0.1.2: row norm, 8-bit product, gradient norm and clipping (0.1.1: dsw_hop2_plan carries its own size, struct_bytes)
 
 // error codes returned by every C-ABI entry point (0 = ok)
 #define DSW_OK 0
@@ -13,6 +13,7 @@
 #define DSW_ERR_WORKSPACE (-3)
 #define DSW_ERR_LAUNCH (-4)
 #define DSW_ERR_ALIGN (-5)
+#define DSW_ERR_OVERLAP (-6)
 
 #define DSW_F32 0
 #define DSW_BF16 1

@@ -24,6 +24,7 @@ _f32p = ctypes.c_void_p
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _int = ctypes.c_int
 
 # name -> (restype, argtypes): exactly the declarations of include/dsw_hip.h
@@ -102,6 +103,16 @@ SIGNATURES = {
         [_i32p, _i32p, _f32p, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
          _i64, _int, _vp, _vp],
     ),
+    "dsw_rmsnorm_fwd": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _f32p, _i64, _i64, _f32, _int, _vp]),
+    "dsw_rmsnorm_fwd_fp8": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _f32p, _i64, _vp, _i64, _i64, _f32, _int, _vp]),
+    "dsw_quant_fp8": (_int, [_vp, _i64, _vp, _f32p, _i64, _i64, _i64, _int, _vp]),
+    "dsw_quant_fp8_weight": (_int, [_vp, _i64, _i64, _vp, _f32p, _i64, _i64, _int, _vp]),
+    "dsw_rmsnorm_bwd_workspace_bytes": (_i64, [_i64, _i64, _int]),
+    "dsw_rmsnorm_bwd": (_int, [_vp, _vp, _vp, _i64, _vp, _f32p, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
+    "dsw_fp8_mix_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "dsw_fp8_mix": (_int, [_vp, _i64, _f32p, _i64, _i64, _vp, _i64, _f32p, _vp, _vp, _i64, _i64, _i64, _int, _vp, _i64, _vp]),
+    "dsw_grad_norm_workspace_bytes": (_i64, []),
+    "dsw_grad_norm_clip": (_int, [_int, _vp, _vp, _vp, _vp, _f64, _f64, _f32p, _vp, _i64, _vp]),
 }
 
 _lib = None
@@ -144,7 +155,8 @@ def load():
 
 ROLE_NAMES = {1: "spmm", 2: "spmm2", 3: "spmm_staged", 4: "basis_fwd", 5: "basis_adj", 6: "mix_fwd", 7: "fwd_one_launch",
               8: "bwd_gemm_fused", 9: "bwd_dgrad", 10: "bwd_wgrad", 11: "zmix", 12: "clenshaw_fwd", 13: "elementwise",
-              14: "bwd_fused", 15: "basis_dual", 16: "fwd_hop2_mix", 17: "bwd_dual"}
+              14: "bwd_fused", 15: "basis_dual", 16: "fwd_hop2_mix", 17: "bwd_dual",
+              18: "rmsnorm", 19: "fp8_mix", 20: "grad_norm"}
 
 
 class LaunchTrace:

@@ -39,6 +39,7 @@ extern "C" {
 #define DSW_ERR_WORKSPACE (-3)
 #define DSW_ERR_LAUNCH (-4)
 #define DSW_ERR_ALIGN (-5)
+#define DSW_ERR_OVERLAP (-6)
 
 typedef void* dsw_stream_t; /* hipStream_t */
 
@@ -122,6 +123,9 @@ int dsw_build_flags(void);
 #define DSW_ROLE_BWD_FUSED 14      /* (retired in round 6 with dsw_cheb_dx_one_launch: never emitted) */
 #define DSW_ROLE_FWD_HOP2_MIX 16     /* hop 2 + channel mix + bias of the forward in one launch (one-hop plans) */
 #define DSW_ROLE_BASIS_DUAL 15     /* mix-first backward: Chebyshev basis of dY under L^T (on the output channels) */
+#define DSW_ROLE_RMSNORM 18          /* row norm (aux: rows, C, 0 forward / 1 forward with 8-bit output / 4 backward), 8-bit rows (2), 8-bit weights (3) */
+#define DSW_ROLE_FP8_MIX 19          /* 8-bit product (aux: rows, Fin, Fout) */
+#define DSW_ROLE_GRAD_NORM 20        /* gradient norm and clipping (aux: tensors, segments, 1 with clipping) */
 #define DSW_ROLE_BWD_DUAL 17       /* whole backward in one launch in the dual form (X, dY -> dX, dW, db), + the partial reduce */
 int dsw_trace_begin(int capacity);
 int dsw_trace_end(int32_t* call, int32_t* roles, int32_t* aux0, int32_t* aux1, int32_t* aux2, float* us, char* names,
@@ -404,6 +408,58 @@ int dsw_maxval_unpool_fwd(const int32_t* sel, const void* X, void* Y, void* work
 /* Its backward (autograd of index_put):  dX[b,d,f] = dY[b, sel[b,d,f], f]. */
 int dsw_maxval_unpool_bwd(const int32_t* sel, const void* dY, void* dX, int64_t B, int64_t v_coarse, int64_t v_fine,
                           int64_t C, int dtype, dsw_stream_t stream);
+
+/* Root-mean-square norm of the C channels of every row, with the residual's addition in front:
+ *     h = x + r,  rstd = (mean_c h^2 + eps)^(-1/2),  y = h rstd w
+ * X / R: rows of C channels, ldx / ldr elements apart (channel slices of wider tensors), any element alignment; Y, H: dense;
+ * W: [C].  R and H: both NULL (no residual) or both given (H = the sum, rounded to dtype; Y comes from the unrounded sum).
+ * rstd: fp32 [rows] for the backward pass, or NULL.  Sums are fp32.  1 <= C <= 2^24, rows < 2^31 (0: nothing is launched). */
+int dsw_rmsnorm_fwd(const void* X, int64_t ldx, const void* R, int64_t ldr, const void* W, void* Y, void* H, float* rstd,
+                    int64_t rows, int64_t C, float eps, int dtype, dsw_stream_t stream);
+
+/* The same with an 8-bit output: Q [rows][C] OCP e4m3 (largest finite value 448) and one fp32 scale per row and block of 128
+ * channels (the last block may be shorter), S[block * s_ld + row] with s_ld >= rows:
+ *     s_b = max(max|y_b| / 448, 2^-126),   q = e4m3(y / s_b), to nearest even.   A NaN in a block makes its scale a NaN. */
+int dsw_rmsnorm_fwd_fp8(const void* X, int64_t ldx, const void* R, int64_t ldr, const void* W, void* Q, float* S, int64_t s_ld,
+                        void* H, int64_t rows, int64_t C, float eps, int dtype, dsw_stream_t stream);
+
+/* 8-bit rows without a norm in front (q = e4m3(x / s_b)), and 8-bit weights: W(k, n) at element k * stride_in + n * stride_out
+ * -> Q [Fout][Fin], S [ceil(Fout / 128)][ceil(Fin / 128)], one scale per 128 x 128 block. */
+int dsw_quant_fp8(const void* X, int64_t ldx, void* Q, float* S, int64_t s_ld, int64_t rows, int64_t C, int dtype,
+                  dsw_stream_t stream);
+int dsw_quant_fp8_weight(const void* W, int64_t stride_in, int64_t stride_out, void* Q, float* S, int64_t Fin, int64_t Fout,
+                         int dtype, dsw_stream_t stream);
+
+/* Backward of dsw_rmsnorm_fwd.  G = dL/dy, D = dL/dh or NULL, H = what the forward stored (or its input where there was no
+ * residual; rows ldh elements apart), rstd as stored:
+ *     dX = D + rstd (G w - xhat mean_c(G w xhat)),  xhat = h rstd     (the gradient of x AND of r);     dW = sum_rows G xhat
+ * dX or dW may be NULL.  G, D, dX dense.  The workspace (dsw_rmsnorm_bwd_workspace_bytes) is needed for dW; no atomics: equal
+ * inputs give equal bits.  rows == 0: dW = 0. */
+int64_t dsw_rmsnorm_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype);
+int dsw_rmsnorm_bwd(const void* G, const void* D, const void* H, int64_t ldh, const void* W, const float* rstd, void* dX, void* dW,
+                    void* workspace, int64_t workspace_bytes, int64_t rows, int64_t C, int dtype, dsw_stream_t stream);
+
+/* Per-node linear map of e4m3 rows and e4m3 weights, a scale per block of 128:
+ *     Y[m, n] = sum_b XS[m * xs_row + b * xs_blk] * WS[(n / 128) * ceil(K / 128) + b] * sum_{k in block b} X[m, k] W[n, k] + bias[n]
+ * X: M rows of K bytes, ldx apart; W: N rows of K bytes, ldw apart; bias [N] of dtype or NULL; Y [M][N] dense, dtype = its type.
+ * Any K, N >= 1 and alignments; the order of every sum is fixed by the sizes.  fp32 output: exact products, fp32 sums.  bf16
+ * output: the 8-bit matrix instructions, which within 8 neighbouring k drop what lies 13 bits below the largest product, then sum
+ * in fp32: each group of 8 loses at most 7 * 2^-13 of its largest product (relative 2-norm of random rows: 1.5e-5). */
+int64_t dsw_fp8_mix_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int dsw_fp8_mix(const void* X, int64_t ldx, const float* XS, int64_t xs_row, int64_t xs_blk, const void* W, int64_t ldw,
+                const float* WS, const void* bias, void* Y, int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
+                int64_t workspace_bytes, dsw_stream_t stream);
+
+/* Norm of n gradient tensors taken together, and their clipping (HOST arrays of n device pointers, element counts, dtypes):
+ *     N = (sum |g|^p)^(1/p), norm_type p = 1, 2 or infinity;   c = min(1, max_norm / (N + 1e-6));   outs[i] = c * grads[i]
+ * norm: device, fp32.  outs NULL: the norm alone; outs[i] == grads[i]: in place (nothing is written where c == 1).  Written
+ * ranges must overlap nothing but the gradient they replace (DSW_ERR_OVERLAP: a tensor listed twice).  A NaN or infinite
+ * gradient gives a NaN / infinite norm.  Sums are held in 64 bits and their order is fixed by the sizes and addresses' adjacency.
+ * The arrays are read during the call only; workspace: dsw_grad_norm_workspace_bytes(), 8-byte aligned. */
+int64_t dsw_grad_norm_workspace_bytes(void);
+int dsw_grad_norm_clip(int n, const void* const* grads, void* const* outs, const int64_t* numel, const int32_t* dtypes,
+                       double norm_type, double max_norm, float* norm, void* workspace, int64_t workspace_bytes,
+                       dsw_stream_t stream);
 
 #ifdef __cplusplus
 }
