@@ -19,6 +19,8 @@ typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 struct __attribute__((packed, aligned(1))) Any16 { u32x4 v; };
 
+constexpr int64_t MIX_LD_MAX = (1 << 24) - 1;      // a tile's rows are reached by 32-bit offsets
+
 struct MixArgs {
     const uint8_t* X; const float* XS; const uint8_t* W; const float* WS; const void* bias; void* Y;
     long ldx, ldw, xs_row, xs_blk;      // element strides; XS[m * xs_row + b * xs_blk], WS[nb * KB + b]
@@ -81,69 +83,268 @@ static __device__ __forceinline__ void store_out(void* p, long i, float v) {
     else static_cast<float*>(p)[i] = v;
 }
 
-// Any sizes, strides and alignments: 128 x 128 outputs per workgroup of four waves (64 x 64 each), one scale block per step,
-// operands through LDS (16-byte chunks, chunk c of row r at place c ^ (r & 7): the reads of a wave spread over all banks)
-constexpr int MG_TILE = 128;
-template <bool BF16>
-__global__ __launch_bounds__(256) void fp8_mix_any_kernel(const MixArgs P) {
-    __shared__ u32x4 sw[MG_TILE * 8], sx[MG_TILE * 8];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n0 = blockIdx.x * MG_TILE, m0 = blockIdx.y * MG_TILE;
-    const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64;
+// One lane's 16 bytes global memory -> LDS (lane l of the wave writes LDS byte `lds` + 16 l); waited for by hand (vmcnt).
+static __device__ __forceinline__ void load_to_lds(const uint8_t* base, uint32_t off, uint32_t lds) {
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "v"(off), "s"(base), "s"(lds) : "memory");
+}
+
+// ---- many rows: tiles of (16 NT WN) outputs n x (16 MT WM) rows m per workgroup of WN x WM waves -----------------------------
+// Operands travel through LDS, one scale block (128 bytes of every row) per step, two stages: while a block is multiplied the
+// next one is on its way.  Row r of a stage is 128 bytes, its 16-byte chunk c sits at place c ^ f(r), so that the 16 rows a
+// fragment reads spread over the banks.  Which n a row of the matrix instruction stands for is free: row r of tile t of a wave is
+// n = 4 NT (r / 4) + 4 t + r % 4, so that a lane ends with 4 NT neighbouring outputs of one row m and stores whole 16 bytes.
+// DMA: 16-byte aligned rows of whole 16-byte chunks go to LDS directly; otherwise through registers.
+template <int NT>
+static __device__ __forceinline__ int w_place(int row) { return (row & 3) | (((row / (4 * NT)) & 1) << 2); }
+
+template <int NT, int MT, int WN, int WM, bool BF16, bool DMA>
+__global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArgs P, const int tiles_n, const int tiles_m) {
+    constexpr bool WIDE = !BF16;
+    constexpr int WAVES = WN * WM, BN = 16 * NT * WN, BM = 16 * MT * WM, ROWS = BN + BM, PIECES = ROWS / 8 / WAVES;
+    static_assert(ROWS % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "a wave's pieces lie in one operand each");
+    static_assert(128 % (16 * NT) == 0, "a wave's outputs share a row of weight scales");
+    extern __shared__ u32x4 lds[];                     // [2][ROWS][8]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // tiles: each of the 8 dies takes a contiguous run of them (blocks go round the dies), 8 row tiles deep
+    const int T = tiles_n * tiles_m, per = (T + 7) >> 3;
+    const int t_id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (t_id >= T) return;
+    const int deep = 8, band = t_id / (deep * tiles_n), in = t_id - band * deep * tiles_n;
+    const int high = tiles_m - band * deep < deep ? tiles_m - band * deep : deep;
+    const int n0 = (in / high) * BN, m0 = (band * deep + in % high) * BM;
+    const int wn = (wave % WN) * 16 * NT, wm = (wave / WN) * 16 * MT;
     const int r16 = lane & 15, g = lane >> 4;
-    f32x4 acc[4][4];
+
+    // this lane's share of a stage: PIECES chunks, the first BN / 8 pieces are weight rows
+    uint32_t off[PIECES];
+    const uint8_t* const wbase = P.W + (long)n0 * P.ldw;
+    const uint8_t* const xbase = P.X + (long)m0 * P.ldx;
+    auto piece_row = [&](int i) { return (wave + i * WAVES) * 8 + (lane >> 3); };
+    auto piece_chunk = [&](int i) {
+        const int row = piece_row(i);
+        return row < BN ? (lane & 7) ^ w_place<NT>(row) : (lane & 7) ^ ((row - BN) & 7);
+    };
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < PIECES; ++i) {
+        const int row = piece_row(i);
+        if (row < BN) off[i] = (uint32_t)((n0 + row < P.N ? row : P.N - 1 - n0) * P.ldw) + piece_chunk(i) * 16;
+        else off[i] = (uint32_t)((m0 + row - BN < P.M ? row - BN : P.M - 1 - m0) * P.ldx) + piece_chunk(i) * 16;
+    }
+    const int whole = P.K >> 7, tail = P.K & 127;      // whole blocks, bytes of the last one
+    u32x4 held[DMA ? 1 : PIECES];
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    auto fetch = [&](int b, int stage) {
+        if constexpr (DMA) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int b = 0; b < P.KB; ++b) {
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int e = q * 256 + threadIdx.x, r = e >> 3, c = e & 7;
-            const u32x4 z = {0u, 0u, 0u, 0u};
-            sw[r * 8 + (c ^ (r & 7))] = n0 + r < P.N ? row_chunk(P.W + (long)(n0 + r) * P.ldw, b * 128 + c * 16, P.K) : z;
-            sx[r * 8 + (c ^ (r & 7))] = m0 + r < P.M ? row_chunk(P.X + (long)(m0 + r) * P.ldx, b * 128 + c * 16, P.K) : z;
-        }
-        __syncthreads();
-        const int nb = (n0 + wn) / 128;
-        const float ws = n0 + wn < P.N ? P.WS[(long)nb * P.KB + b] : 0.f;
-        Frag<!BF16> fa[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = wn + i * 16 + r16;
-            const u32x4 lo = sw[r * 8 + (g ^ (r & 7))], hi = sw[r * 8 + ((g + 4) ^ (r & 7))];
-            fa[i] = make_frag<!BF16>(lo, hi);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = wm + j * 16 + r16;
-            const u32x4 lo = sx[r * 8 + (g ^ (r & 7))], hi = sx[r * 8 + ((g + 4) ^ (r & 7))];
-            const Frag<!BF16> fb = make_frag<!BF16>(lo, hi);
-            const int m = m0 + r < P.M ? m0 + r : P.M - 1;
-            const float s = ws * P.XS[(long)m * P.xs_row + (long)b * P.xs_blk];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x4 p = block_product<!BF16>(fa[i], fb);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[i][j][k] = fmaf(p[k], s, acc[i][j][k]);
+            for (int i = 0; i < PIECES; ++i) {
+                const bool w = i < BN / 8 / WAVES;
+                uint32_t o = off[i];
+                if (b == whole) { const int c = piece_chunk(i); o = c * 16 < tail ? o : o - c * 16; }    // (chunks behind the row: cleared below)
+                load_to_lds((w ? wbase : xbase) + (long)b * 128, o, lds0 + (uint32_t)((stage * ROWS + (wave + i * WAVES) * 8) * 128));
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const uint8_t* p = (i < BN / 8 / WAVES ? wbase : xbase) + off[i] + (long)b * 128;
+                held[i] = row_chunk(p, 0, P.K - b * 128 - piece_chunk(i) * 16);
+            }
+        }
+    };
+    auto store_held = [&](int stage) {
+        if constexpr (!DMA) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) lds[(stage * ROWS + piece_row(i)) * 8 + (lane & 7)] = held[i];
+        }
+    };
+
+    const float* xs[MT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        const int m = m0 + wm + 16 * j + r16;
+        xs[j] = P.XS + (long)(m < P.M ? m : P.M - 1) * P.xs_row;
+    }
+    const int nb = (n0 + wn) >> 7, nb_last = (P.N - 1) >> 7;
+    const float* const ws = P.WS + (long)(nb < nb_last ? nb : nb_last) * P.KB;
+
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float sx[MT], sw = ws[0];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) sx[j] = xs[j][0];
+    fetch(0, 0);
+    store_held(0);
+    for (int b = 0; b < P.KB; ++b) {
+        const int stage = b & 1;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();                               // the block has landed; the other stage is no longer read
+        if (DMA && b == whole) {                       // the last block is short: clear what lies behind the rows
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+                if (piece_chunk(i) * 16 >= tail) lds[(stage * ROWS + piece_row(i)) * 8 + (lane & 7)] = u32x4{0u, 0u, 0u, 0u};
+            __syncthreads();
+        }
+        float s[MT];
+#pragma unroll
+        for (int j = 0; j < MT; ++j) s[j] = sw * sx[j];
+        if (b + 1 < P.KB) {
+            sw = ws[b + 1];
+#pragma unroll
+            for (int j = 0; j < MT; ++j) sx[j] = xs[j][(long)(b + 1) * P.xs_blk];
+            fetch(b + 1, stage ^ 1);
+        }
+        const u32x4* const base = lds + stage * ROWS * 8;
+        Frag<WIDE> fx[MT];
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            const int r = BN + wm + 16 * j + r16, f = r16 & 7;
+            fx[j] = make_frag<WIDE>(base[r * 8 + (g ^ f)], base[r * 8 + ((g + 4) ^ f)]);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int r = wn + 4 * NT * (r16 >> 2) + 4 * t + (r16 & 3), f = w_place<NT>(r);
+            const Frag<WIDE> fw = make_frag<WIDE>(base[r * 8 + (g ^ f)], base[r * 8 + ((g + 4) ^ f)]);
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                const f32x4 p = block_product<WIDE>(fw, fx[j]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[t][j][k] = fmaf(p[k], s[j], acc[t][j][k]);
+            }
+        }
+        if (b + 1 < P.KB) store_held(stage ^ 1);
+    }
+
+    const int n = n0 + wn + 4 * NT * g;
+    float add[4 * NT];
+#pragma unroll
+    for (int k = 0; k < 4 * NT; ++k) add[k] = P.bias != nullptr && n + k < P.N ? load_out<BF16>(P.bias, n + k) : 0.f;
+    const bool vec = n + 4 * NT <= P.N && P.N % 8 == 0 && ((uintptr_t)P.Y & 15) == 0;
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        const int m = m0 + wm + 16 * j + r16;
+        if (m >= P.M) continue;
+        const long at = (long)m * P.N + n;
+        if (vec) {
+            if constexpr (BF16) {
+#pragma unroll
+                for (int t = 0; t < NT; t += 2) {
+                    u32x4 v;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int e = t * 4 + 2 * q;
+                        v[q] = f32_to_bf16(acc[e / 4][j][e % 4] + add[e]) | (uint32_t)f32_to_bf16(acc[e / 4][j][e % 4 + 1] + add[e + 1]) << 16;
+                    }
+                    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(P.Y) + at + 4 * t) = v;
+                }
+            } else {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    f32x4 v = acc[t][j];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) v[q] += add[4 * t + q];
+                    *reinterpret_cast<f32x4*>(static_cast<float*>(P.Y) + at + 4 * t) = v;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (n + 4 * t + q < P.N) store_out<BF16>(P.Y, at + 4 * t + q, acc[t][j][q] + add[4 * t + q]);
+        }
+    }
+}
+
+// ---- few rows: 16 outputs n x 16 MT rows m per workgroup; the waves share the blocks of K ------------------------------------
+// Bound by reading the weights: every wave reads the 16 weight rows of its blocks straight into registers (16 bytes per lane and
+// load, any alignment), the partial sums of the waves are joined in wave order through LDS.
+constexpr int FEW_WAVES = 8;
+template <int MT, bool BF16>
+__global__ __launch_bounds__(64 * FEW_WAVES) void fp8_mix_few_kernel(const MixArgs P) {
+    constexpr bool WIDE = !BF16;
+    __shared__ float part[FEW_WAVES][MT * 4][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
+    const int r16 = lane & 15, g = lane >> 4;
+    const uint8_t* const w = P.W + (long)(n0 + r16 < P.N ? n0 + r16 : P.N - 1) * P.ldw;
+    const uint8_t* x[MT];
+    const float* xs[MT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        const int m = m0 + 16 * j + r16 < P.M ? m0 + 16 * j + r16 : P.M - 1;
+        x[j] = P.X + (long)m * P.ldx;
+        xs[j] = P.XS + (long)m * P.xs_row;
+    }
+    const float* const ws = P.WS + (long)(n0 >> 7) * P.KB;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int b = wave; b < P.KB; b += FEW_WAVES) {
+        const int k = b * 128 + g * 16;
+        const Frag<WIDE> fw = make_frag<WIDE>(row_chunk(w, k, P.K), row_chunk(w, k + 64, P.K));
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            const Frag<WIDE> fx = make_frag<WIDE>(row_chunk(x[j], k, P.K), row_chunk(x[j], k + 64, P.K));
+            const float s = ws[b] * xs[j][(long)b * P.xs_blk];
+            const f32x4 p = block_product<WIDE>(fw, fx);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[j][q] = fmaf(p[q], s, acc[j][q]);
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < MT; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int m = m0 + wm + j * 16 + r16;
+        for (int q = 0; q < 4; ++q) part[wave][4 * j + q][lane] = acc[j][q];
+    __syncthreads();
+    // output (n, m) of the tile: lane 16 (n / 4) + m % 16 of register 4 (m / 16) + n % 4
+    for (int e = threadIdx.x; e < 256 * MT; e += 64 * FEW_WAVES) {
+        const int n = e & 15, m = e >> 4;
+        const int reg = 4 * (m >> 4) + (n & 3), l = 16 * (n >> 2) + (m & 15);
+        float v = 0.f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int n = n0 + wn + i * 16 + g * 4 + k;
-                if (m < P.M && n < P.N) {
-                    const float v = acc[i][j][k] + (P.bias != nullptr ? load_out<BF16>(P.bias, n) : 0.f);
-                    store_out<BF16>(P.Y, (long)m * P.N + n, v);
-                }
-            }
+        for (int q = 0; q < FEW_WAVES; ++q) v += part[q][reg][l];
+        if (m0 + m < P.M && n0 + n < P.N) {
+            if (P.bias != nullptr) v += load_out<BF16>(P.bias, n0 + n);
+            store_out<BF16>(P.Y, (long)(m0 + m) * P.N + n0 + n, v);
         }
+    }
+}
+
+template <int NT, int MT, int WN, int WM, bool BF16, bool DMA>
+static int launch_tile(const MixArgs& a, hipStream_t s) {
+    constexpr int BN = 16 * NT * WN, BM = 16 * MT * WM;
+    const int tn = (a.N + BN - 1) / BN, tm = (a.M + BM - 1) / BM;
+    const int lds = 2 * (BN + BM) * 128;
+    auto* kernel = fp8_mix_tile_kernel<NT, MT, WN, WM, BF16, DMA>;
+    if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+        return DSW_ERR_LAUNCH;
+    const long per = ((long)tn * tm + 7) / 8;
+    DSW_LAUNCH(kernel, dim3((unsigned)(per * 8)), dim3(64 * WN * WM), lds, s, a, tn, tm);
+    return dsw_check_launch();
+}
+template <bool BF16>
+static int launch_few(const MixArgs& a, hipStream_t s) {
+    const unsigned gn = (unsigned)((a.N + 15) / 16);
+#define FEW(MT_) DSW_LAUNCH((fp8_mix_few_kernel<MT_, BF16>), dim3(gn, (unsigned)((a.M + 16 * MT_ - 1) / (16 * MT_))), dim3(64 * FEW_WAVES), 0, s, a)
+    if (a.M <= 16) FEW(1);
+    else if (a.M <= 32) FEW(2);
+    else FEW(4);
+#undef FEW
+    return dsw_check_launch();
+}
+template <bool BF16>
+static int launch_mix(const MixArgs& a, hipStream_t s) {
+    const bool dma = a.K % 16 == 0 && a.ldx % 16 == 0 && a.ldw % 16 == 0 && dsw_aligned16(a.X) && dsw_aligned16(a.W);
+    if (a.M <= 64 || (long)((a.M + 127) / 128) * ((a.N + 127) / 128) < 64) return launch_few<BF16>(a, s);
+    if (!dma) return launch_tile<4, 4, 2, 2, BF16, false>(a, s);
+    if constexpr (BF16) {
+        if ((long)((a.M + 255) / 256) * ((a.N + 255) / 256) >= 256) return launch_tile<8, 4, 2, 4, BF16, true>(a, s);
+    }
+    return launch_tile<4, 4, 2, 2, BF16, true>(a, s);
 }
 
 }  // namespace
@@ -151,7 +352,7 @@ __global__ __launch_bounds__(256) void fp8_mix_any_kernel(const MixArgs P) {
 extern "C" {
 
 int64_t dsw_fp8_mix_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    if (M < 0 || N < 1 || K < 1 || M > 0x7fffffff - 256 || N > (1 << 22) || K > (1 << 24)) return DSW_ERR_BAD_ARG;
+    if (M < 0 || N < 1 || K < 1 || M > 0x7fffffff - 256 || N > (1 << 22) || K > MIX_LD_MAX) return DSW_ERR_BAD_ARG;
     return 0;
 }
 
@@ -160,7 +361,7 @@ int dsw_fp8_mix(const void* X, int64_t ldx, const float* XS, int64_t xs_row, int
                 int64_t workspace_bytes, dsw_stream_t stream) {
     if (dtype != DSW_F32 && dtype != DSW_BF16) return DSW_ERR_BAD_DTYPE;
     const int64_t need = dsw_fp8_mix_workspace_bytes(M, N, K);
-    if (need < 0 || ldx < K || ldw < K || xs_row < 0 || xs_blk < 0) return DSW_ERR_BAD_ARG;
+    if (need < 0 || ldx < K || ldw < K || ldx > MIX_LD_MAX || ldw > MIX_LD_MAX || xs_row < 0 || xs_blk < 0) return DSW_ERR_BAD_ARG;
     if (M == 0) return DSW_OK;
     if (!X || !XS || !W || !WS || !Y) return DSW_ERR_BAD_ARG;
     if (need > 0 && (!workspace || workspace_bytes < need)) return DSW_ERR_WORKSPACE;
@@ -168,11 +369,7 @@ int dsw_fp8_mix(const void* X, int64_t ldx, const float* XS, int64_t xs_row, int
     DswTraceScope trace_(s, DSW_ROLE_FP8_MIX, M, K, N);
     const MixArgs a{(const uint8_t*)X, XS, (const uint8_t*)W, WS, bias, Y, (long)ldx, (long)ldw, (long)xs_row, (long)xs_blk,
                     (int)M, (int)N, (int)K, (int)((K + 127) / 128)};
-    const dim3 grid((unsigned)((N + MG_TILE - 1) / MG_TILE), (unsigned)((M + MG_TILE - 1) / MG_TILE));
-    if (grid.y > 65535u * 4u) return DSW_ERR_BAD_ARG;
-    if (dtype == DSW_BF16) DSW_LAUNCH(fp8_mix_any_kernel<true>, grid, dim3(256), 0, s, a);
-    else DSW_LAUNCH(fp8_mix_any_kernel<false>, grid, dim3(256), 0, s, a);
-    return dsw_check_launch();
+    return dtype == DSW_BF16 ? launch_mix<true>(a, s) : launch_mix<false>(a, s);
 }
 
 }  // extern "C"

@@ -15,7 +15,8 @@ namespace {
 constexpr int GN_THREADS = 256;
 constexpr int GN_TENSORS = 144;            // segments per launch: their table travels as a kernel argument (< 4 KB), so a captured
                                            // graph owns its copy and no host buffer has to outlive the call
-constexpr int GN_CHUNK = 256 * 64;         // elements of a workgroup's step
+constexpr int GN_AHEAD = 4;                // 16-byte loads of a thread in flight
+constexpr int GN_CHUNK = 256 * 32;         // elements of a workgroup's step: 4 (bf16) or 8 (fp32) loads of each thread
 constexpr int GN_BLOCKS = 1024;            // partial sums of one launch at most
 constexpr int GN_MAX_PARTS = 16 * 1024;    // partial sums of one call at most
 
@@ -61,7 +62,20 @@ template <int P, bool BF16>
 static __device__ __forceinline__ double chunk_sum(const char* g, int n, double s) {
     using Rw = Row<BF16>;
     constexpr int V = Rw::V;
-    for (int i = threadIdx.x * V; i < n; i += GN_THREADS * V) {
+    int i = threadIdx.x * V;
+    for (; i + (GN_AHEAD - 1) * GN_THREADS * V + V <= n; i += GN_AHEAD * GN_THREADS * V) {
+        typename Rw::u32x4 t[GN_AHEAD];
+#pragma unroll
+        for (int q = 0; q < GN_AHEAD; ++q) t[q] = Rw::raw(g + (long)(i + q * GN_THREADS * V) * Rw::E);
+#pragma unroll
+        for (int q = 0; q < GN_AHEAD; ++q) {
+            float v[V];
+            Rw::unpack(t[q], v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) s = fold<P>(s, v[j]);
+        }
+    }
+    for (; i < n; i += GN_THREADS * V) {
         float v[V];
         Rw::load(g + (long)i * Rw::E, n - i, v);
 #pragma unroll
@@ -97,7 +111,21 @@ template <bool BF16>
 static __device__ __forceinline__ void chunk_scale(const char* g, char* o, int n, float c) {
     using Rw = Row<BF16>;
     constexpr int V = Rw::V;
-    for (int i = threadIdx.x * V; i < n; i += GN_THREADS * V) {
+    int i = threadIdx.x * V;
+    for (; i + (GN_AHEAD - 1) * GN_THREADS * V + V <= n; i += GN_AHEAD * GN_THREADS * V) {
+        typename Rw::u32x4 t[GN_AHEAD];
+#pragma unroll
+        for (int q = 0; q < GN_AHEAD; ++q) t[q] = Rw::raw(g + (long)(i + q * GN_THREADS * V) * Rw::E);
+#pragma unroll
+        for (int q = 0; q < GN_AHEAD; ++q) {
+            float v[V];
+            Rw::unpack(t[q], v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] *= c;
+            Rw::put_raw(o + (long)(i + q * GN_THREADS * V) * Rw::E, Rw::pack(v));
+        }
+    }
+    for (; i < n; i += GN_THREADS * V) {
         float v[V];
         Rw::load(g + (long)i * Rw::E, n - i, v);
 #pragma unroll

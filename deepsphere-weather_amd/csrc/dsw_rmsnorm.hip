@@ -316,19 +316,28 @@ __global__ __launch_bounds__(RN_THREADS) void rmsnorm_bwd_long_dw_kernel(const N
     P.part[(long)blockIdx.y * P.C + c] = s;
 }
 
-// dw[c] = sum over the workgroups' rows of part, in a fixed order: 32 columns per workgroup, 8 threads per column
+// dw[c] = sum over the workgroups' rows of part, in a fixed order: 16 columns per workgroup, 16 threads per column, each with
+// four chains of its own (a chain of dependent loads is what such a short kernel spends its time on)
 template <bool BF16>
 __global__ __launch_bounds__(RN_THREADS) void rmsnorm_dw_kernel(const float* part, int nparts, int C, char* dW) {
-    __shared__ float red[8][33];
-    const int k = threadIdx.x & 31, g = threadIdx.x >> 5, c = blockIdx.x * 32 + k;
-    float s = 0.f;
-    if (c < C) for (int p = g; p < nparts; p += 8) s += part[(long)p * C + c];
-    red[g][k] = s;
+    __shared__ float red[16][17];
+    const int k = threadIdx.x & 15, g = threadIdx.x >> 4, c = blockIdx.x * 16 + k;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < C) {
+        int p = g;
+#pragma unroll 4
+        for (; p + 48 < nparts; p += 64)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s[q] += part[(long)(p + 16 * q) * C + c];
+        for (int q = 0; p < nparts; p += 16, ++q) s[q & 3] += part[(long)p * C + c];
+    }
+    red[g][k] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
     if (g == 0 && c < C) {
+        float v = red[0][k];
 #pragma unroll
-        for (int q = 1; q < 8; ++q) s += red[q][k];
-        Row<BF16>::put(dW + (long)c * Row<BF16>::E, s);
+        for (int q = 1; q < 16; ++q) v += red[q][k];
+        Row<BF16>::put(dW + (long)c * Row<BF16>::E, v);
     }
 }
 
@@ -399,7 +408,7 @@ static int launch_bwd(const NormBwdArgs& a, char* dW, hipStream_t s) {
 #undef CASE
     }
     if (a.part != nullptr)
-        DSW_LAUNCH(rmsnorm_dw_kernel<BF16>, dim3((unsigned)((a.C + 31) / 32)), dim3(RN_THREADS), 0, s, a.part, (int)blocks, a.C, dW);
+        DSW_LAUNCH(rmsnorm_dw_kernel<BF16>, dim3((unsigned)((a.C + 15) / 16)), dim3(RN_THREADS), 0, s, a.part, (int)blocks, a.C, dW);
     return dsw_check_launch();
 }
 

@@ -42,6 +42,8 @@ struct Row {
         }
         return t;
     }
+    static __device__ __forceinline__ u32x4 raw(const char* p) { return reinterpret_cast<const Any*>(p)->v; }
+    static __device__ __forceinline__ void put_raw(char* p, const u32x4 t) { reinterpret_cast<Any*>(p)->v = t; }
     // channels [0, n) of the 16 bytes at p; the others come back as zero (n >= V: all of them)
     static __device__ __forceinline__ void load(const char* p, int n, float (&v)[V]) {
         if (n >= V) {

@@ -329,8 +329,31 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(t):
+    """Handle of the current stream of t's device (without building a Stream object where torch has a way: 0.1 against 2 us)."""
+    if _raw_stream is not None:
+        return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+class _NoGuard:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_no_guard = _NoGuard()
+
+
+def _guard(t):
+    """``torch.cuda.device(t.device)``, which costs nothing where that is the current device."""
+    i = t.get_device()
+    return _no_guard if i == torch.cuda.current_device() else torch.cuda.device(i)
 
 
 def _plan_ptr(op, x, channels=None):
@@ -685,7 +708,7 @@ class _HipBackend:
         y = torch.empty(xt.shape, dtype=xt.dtype, device=xt.device)
         h = torch.empty(xt.shape, dtype=xt.dtype, device=xt.device) if r is not None else None
         rstd = torch.empty((rows,), dtype=torch.float32, device=xt.device) if need_rstd else None
-        with torch.cuda.device(xt.device):
+        with _guard(xt):
             rc = lib.dsw_rmsnorm_fwd(xt.data_ptr(), ldx, None if r is None else r[0].data_ptr(), 0 if r is None else r[2],
                                      w.data_ptr(), y.data_ptr(), _ptr(h), _ptr(rstd), rows, C, eps, _DTYPES[xt.dtype], _stream(xt))
         _native.check(rc, "dsw_rmsnorm_fwd")
@@ -702,7 +725,7 @@ class _HipBackend:
             if nb < 0:
                 _native.check(nb, "dsw_rmsnorm_bwd_workspace_bytes")
             ws = torch.empty((nb,), dtype=torch.uint8, device=ht.device)
-        with torch.cuda.device(ht.device):
+        with _guard(ht):
             rc = lib.dsw_rmsnorm_bwd(g.data_ptr(), _ptr(d), ht.data_ptr(), ldh, w.data_ptr(), rstd.data_ptr(), _ptr(dx), _ptr(dw),
                                      _ptr(ws), nb, rows, C, _DTYPES[ht.dtype], _stream(ht))
         _native.check(rc, "dsw_rmsnorm_bwd")
@@ -722,7 +745,7 @@ class _HipBackend:
         (xt, rows, ldx), C = x, w.numel()
         q, s, scale = self._fp8_rows(xt, rows, C)
         h = torch.empty(xt.shape, dtype=xt.dtype, device=xt.device) if r is not None else None
-        with torch.cuda.device(xt.device):
+        with _guard(xt):
             rc = lib.dsw_rmsnorm_fwd_fp8(xt.data_ptr(), ldx, None if r is None else r[0].data_ptr(), 0 if r is None else r[2],
                                          w.data_ptr(), q.data_ptr(), s.data_ptr(), rows, _ptr(h), rows, C, eps,
                                          _DTYPES[xt.dtype], _stream(xt))
@@ -733,7 +756,7 @@ class _HipBackend:
         lib = _native.load()
         xt, rows, ldx = x
         q, s, scale = self._fp8_rows(xt, rows, C)
-        with torch.cuda.device(xt.device):
+        with _guard(xt):
             rc = lib.dsw_quant_fp8(xt.data_ptr(), ldx, q.data_ptr(), s.data_ptr(), rows, rows, C, _DTYPES[xt.dtype], _stream(xt))
         _native.check(rc, "dsw_quant_fp8")
         return q, scale
@@ -743,7 +766,7 @@ class _HipBackend:
         fin, fout = w.shape
         q = torch.empty((fout, fin), dtype=torch.float8_e4m3fn, device=w.device)
         s = torch.empty((_fp8_blocks(fout), _fp8_blocks(fin)), dtype=torch.float32, device=w.device)
-        with torch.cuda.device(w.device):
+        with _guard(w):
             rc = lib.dsw_quant_fp8_weight(w.data_ptr(), w.stride(0), w.stride(1), q.data_ptr(), s.data_ptr(), fin, fout,
                                           _DTYPES[w.dtype], _stream(w))
         _native.check(rc, "dsw_quant_fp8_weight")
@@ -753,7 +776,7 @@ class _HipBackend:
         lib = _native.load()
         (xt, rows, ldx), (st, s_row, s_blk), (n, k) = x, xs, wq.shape
         y = torch.empty(xt.shape[:-1] + (n,), dtype=dtype, device=xt.device)
-        with torch.cuda.device(xt.device):
+        with _guard(xt):
             nb = int(lib.dsw_fp8_mix_workspace_bytes(rows, n, k))
             if nb < 0:
                 _native.check(nb, "dsw_fp8_mix_workspace_bytes")
@@ -774,7 +797,7 @@ class _HipBackend:
         o = g if outs is grads else None if outs is None else array.array("Q", [t.data_ptr() for t in outs])
         sizes = array.array("q", [t.numel() for t in grads])
         types = array.array("i", [1 if t.dtype is bf16 else 0 for t in grads])
-        with torch.cuda.device(dev):
+        with _guard(norm):
             rc = lib.dsw_grad_norm_clip(len(grads), g.buffer_info()[0], None if o is None else o.buffer_info()[0],
                                         sizes.buffer_info()[0], types.buffer_info()[0], norm_type, max_norm, norm.data_ptr(),
                                         ws.data_ptr(), ws.numel(), _stream(norm))
@@ -1376,6 +1399,8 @@ def _as_rows(t: torch.Tensor, any_last: bool = False):
     wider tensors stay views; any other layout is copied).  ``any_last``: the last axis may have any stride of its own."""
     C = t.shape[-1]
     rows = t.numel() // C if C else 0
+    if t.is_contiguous():
+        return t, rows, C
     sizes, strides = t.shape, t.stride()
     ok = any_last or C == 1 or strides[-1] == 1
     step = want = None
@@ -1573,9 +1598,11 @@ def dense_mix_fp8(x, weight: Fp8Weight, bias: torch.Tensor = None, dtype: torch.
     _one_device(q, x.scale, wq, weight.scale, bias)
     _no_backward("dense_mix_fp8", bias)
     be = _backend_for(q)
-    if wq.stride(1) != 1 or wq.stride(0) < k:
+    if wq.stride(1) != 1 or not k <= wq.stride(0) < 1 << 24:
         wq = wq.contiguous()
     rows = _as_rows(q)
+    if rows[2] >= 1 << 24:
+        rows = _as_rows(q.contiguous())
     st, _, s_row = _as_rows(x.scale, any_last=True)
     return be.fp8_mix(rows, (st, s_row, st.stride(-1)), wq, weight.scale.contiguous(), None if bias is None else bias.contiguous(), dtype)
 

@@ -244,7 +244,7 @@ def _cut(xq, xs, wq, ws):
     """What the 8-bit instruction may drop: it aligns the 8 products of neighbouring k to the largest exponent among them and
     cuts 13 bits below it, so each of the other 7 loses less than 2^-13 of the largest product of its group."""
     K, N = xq.shape[-1], wq.shape[0]
-    lost = torch.zeros(xq.shape[0], N)
+    lost = torch.zeros(xq.shape[0], N, device=xq.device)
     for k in range(0, K, 8):
         x, w = xq[:, k:k + 8].float().abs(), wq[:, k:k + 8].float().abs()
         s = xs[:, k // 128, None] * ws[:, k // 128].repeat_interleave(128)[None, :N]
@@ -278,6 +278,28 @@ def test_product(rows, K, N, dtype):
     want, mag = _mix64(xq, xs, wq, ws, bias)
     y = F.dense_mix_fp8(F.Fp8Rows(xq.to(DEV), _put(xs, True)), weight, bias.to(DEV), dtype=dtype)
     _within(y, want, _mix_tol(want, mag, K, dtype, cut), "y + bias")
+
+
+# many rows: (rows, K, N, bytes behind a row), for the tiles of 128 x 128 and 256 x 256, whole and odd sizes in every direction
+TILE_SIZES = [(1030, 160, 1100, 0), (1024, 512, 1024, 0), (2001, 272, 515, 16), (1030, 301, 1100, 0), (1100, 1000, 1029, 7), (8200, 16, 129, 0),
+              (4100, 400, 4120, 0), (4096, 256, 4096, 0), (5000, 144, 4000, 112)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,K,N,gap", TILE_SIZES)
+def test_product_of_many_rows(rows, K, N, gap, dtype):
+    xq, xs, wq, ws = (t.to(DEV) for t in _mix_inputs(rows, K, N, 6))
+    bx = torch.full((rows, K + gap), 0x7f, dtype=torch.uint8, device=DEV)                      # NaN behind the rows
+    bx[:, :K] = xq.view(torch.uint8)
+    x8 = bx.view(F8)[:, :K]
+    bias = torch.randn(N, generator=_gen(7)).to(dtype).to(DEV)
+    weight = F.Fp8Weight(wq, ws)
+    y = F.dense_mix_fp8(F.Fp8Rows(x8, _put(xs, True)), weight, bias, dtype=dtype)
+    want, mag = _mix64(xq, xs, wq, ws, bias)                                                   # (64-bit product, on the GPU)
+    cut = _cut(xq, xs, wq, ws).cpu() if dtype == torch.bfloat16 else 0.0
+    _within(y, want.cpu(), _mix_tol(want.cpu(), mag.cpu(), K, dtype, cut), "y")
+    again = F.dense_mix_fp8(F.Fp8Rows(x8, xs), weight, bias, dtype=dtype)                      # scales row after row: the same sums
+    assert torch.equal(again, y)
 
 
 @pytest.mark.parametrize("rows", [1, 40, 300])
