@@ -153,6 +153,29 @@ def load():
     return lib
 
 
+_ops = None
+# entries that the compiled tensor binding (csrc/dsw_torch.cpp) calls
+_OPS_ENTRIES = ("dsw_strerror", "dsw_rmsnorm_fwd", "dsw_rmsnorm_fwd_fp8", "dsw_quant_fp8", "dsw_quant_fp8_weight",
+                "dsw_rmsnorm_bwd_workspace_bytes", "dsw_rmsnorm_bwd", "dsw_fp8_mix_workspace_bytes", "dsw_fp8_mix",
+                "dsw_grad_norm_workspace_bytes", "dsw_grad_norm_clip")
+
+
+def ops():
+    """Load (once) and return the tensor binding of the row norm, the 8-bit channel mix and the gradient clipping
+    (``_dsw_torch``, built next to the library), bound to the library that :func:`load` loaded."""
+    global _ops
+    if _ops is None:
+        try:
+            from . import _dsw_torch as mod
+        except ImportError as exc:
+            raise DswNativeError(f"the tensor binding {os.path.join(_HERE, '_dsw_torch.so')} cannot be loaded ({exc}): build it "
+                                 "(run `python -c 'import __graft_entry__ as g; g.build()'` at the repo root)") from exc
+        lib = load()
+        mod.bind({name: ctypes.cast(getattr(lib, name), _vp).value for name in _OPS_ENTRIES})
+        _ops = mod
+    return _ops
+
+
 ROLE_NAMES = {1: "spmm", 2: "spmm2", 3: "spmm_staged", 4: "basis_fwd", 5: "basis_adj", 6: "mix_fwd", 7: "fwd_one_launch",
               8: "bwd_gemm_fused", 9: "bwd_dgrad", 10: "bwd_wgrad", 11: "zmix", 12: "clenshaw_fwd", 13: "elementwise",
               14: "bwd_fused", 15: "basis_dual", 16: "fwd_hop2_mix", 17: "bwd_dual",

@@ -9,6 +9,8 @@ SOURCES = ["dsw_api.hip", "dsw_spmm.hip", "dsw_gemm.hip", "dsw_gemm_x3.hip", "ds
            "dsw_gemm_x3s.hip", "dsw_narrow.hip", "dsw_elementwise.hip", "dsw_pool.hip", "dsw_fwd3.hip", "dsw_spmm1s.hip", "dsw_bwd3d.hip",
            "dsw_rmsnorm.hip", "dsw_fp8_mix.hip", "dsw_grad_norm.hip"]
 OUT = os.path.join(HERE, "libdsw_hip.so")
+BINDING_SOURCE = "dsw_torch.cpp"
+BINDING = os.path.join(HERE, "_dsw_torch.so")
 
 
 def hipcc_path():
@@ -19,16 +21,35 @@ def hipcc_path():
 
 
 def needs_build():
-    if not os.path.exists(OUT):
+    if not os.path.exists(OUT) or not os.path.exists(BINDING):
         return True
-    t = os.path.getmtime(OUT)
+    t = min(os.path.getmtime(OUT), os.path.getmtime(BINDING))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
     deps.append(os.path.join(os.path.dirname(os.path.dirname(HERE)), "include", "dsw_hip.h"))
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
+def build_binding(verbose=True):
+    """Compile the tensor binding (host code only) against the installed torch's headers."""
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    lib = os.path.join(root, "lib")
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_dsw_torch",
+           *[a for d in inc for a in ("-isystem", d)], os.path.join(CSRC, BINDING_SOURCE), "-o", BINDING,
+           "-L" + lib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print("[dsw build]", " ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True, cwd=CSRC)
+    return BINDING
+
+
 def build(force=False, verbose=True):
-    """Compile every .hip translation unit for gfx950 (in parallel) and link libdsw_hip.so."""
+    """Compile every .hip translation unit for gfx950 (in parallel), link libdsw_hip.so, build the tensor binding."""
     if not force and not needs_build():
         return OUT
     from concurrent.futures import ThreadPoolExecutor
@@ -49,8 +70,10 @@ def build(force=False, verbose=True):
         subprocess.run(cmd, check=True, cwd=CSRC)
         return obj
 
-    with ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+    with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
+        binding = ex.submit(build_binding, verbose)
         objs = list(ex.map(compile_one, SOURCES))
+        binding.result()
     cmd = [hipcc_path(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", OUT, *objs]
     if verbose:
         print("[dsw build]", " ".join(cmd), flush=True)

@@ -11,10 +11,7 @@ consumers and no fused route (a ResBlock's input: conv stack + residual map - th
 """
 from __future__ import annotations
 
-import array
-import math
 import weakref
-from operator import attrgetter
 from typing import NamedTuple
 
 import torch
@@ -329,31 +326,8 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
-
 def _stream(t):
-    """Handle of the current stream of t's device (without building a Stream object where torch has a way: 0.1 against 2 us)."""
-    if _raw_stream is not None:
-        return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
-
-
-class _NoGuard:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_no_guard = _NoGuard()
-
-
-def _guard(t):
-    """``torch.cuda.device(t.device)``, which costs nothing where that is the current device."""
-    i = t.get_device()
-    return _no_guard if i == torch.cuda.current_device() else torch.cuda.device(i)
 
 
 def _plan_ptr(op, x, channels=None):
@@ -700,109 +674,6 @@ class _HipBackend:
                                            _DTYPES[dy.dtype], _stream(dy))
         _native.check(rc, "dsw_maxval_unpool_bwd")
         return dx
-
-    def rmsnorm_fwd(self, x, r, w, eps, need_rstd):
-        """``x`` / ``r``: (tensor, rows, element stride between rows) of ``_as_rows``.  Returns (y, h or None, rstd or None)."""
-        lib = _native.load()
-        (xt, rows, ldx), C = x, w.numel()
-        y = torch.empty(xt.shape, dtype=xt.dtype, device=xt.device)
-        h = torch.empty(xt.shape, dtype=xt.dtype, device=xt.device) if r is not None else None
-        rstd = torch.empty((rows,), dtype=torch.float32, device=xt.device) if need_rstd else None
-        with _guard(xt):
-            rc = lib.dsw_rmsnorm_fwd(xt.data_ptr(), ldx, None if r is None else r[0].data_ptr(), 0 if r is None else r[2],
-                                     w.data_ptr(), y.data_ptr(), _ptr(h), _ptr(rstd), rows, C, eps, _DTYPES[xt.dtype], _stream(xt))
-        _native.check(rc, "dsw_rmsnorm_fwd")
-        return y, h, rstd
-
-    def rmsnorm_bwd(self, g, d, h, w, rstd, need_dx, need_dw):
-        lib = _native.load()
-        (ht, rows, ldh), C = h, w.numel()
-        dx = torch.empty(ht.shape, dtype=ht.dtype, device=ht.device) if need_dx else None
-        dw = torch.empty_like(w) if need_dw else None
-        ws, nb = None, 0
-        if need_dw:
-            nb = int(lib.dsw_rmsnorm_bwd_workspace_bytes(rows, C, _DTYPES[ht.dtype]))
-            if nb < 0:
-                _native.check(nb, "dsw_rmsnorm_bwd_workspace_bytes")
-            ws = torch.empty((nb,), dtype=torch.uint8, device=ht.device)
-        with _guard(ht):
-            rc = lib.dsw_rmsnorm_bwd(g.data_ptr(), _ptr(d), ht.data_ptr(), ldh, w.data_ptr(), rstd.data_ptr(), _ptr(dx), _ptr(dw),
-                                     _ptr(ws), nb, rows, C, _DTYPES[ht.dtype], _stream(ht))
-        _native.check(rc, "dsw_rmsnorm_bwd")
-        return dx, dw
-
-    @staticmethod
-    def _fp8_rows(xt, rows, C):
-        """Uninitialised (q, scale): the scales lie block after block with the rows next to each other (what the product
-        reads in whole lines), behind a view of shape [..., blocks]."""
-        blocks = _fp8_blocks(C)
-        q = torch.empty(xt.shape, dtype=torch.float8_e4m3fn, device=xt.device)
-        s = torch.empty((blocks, rows), dtype=torch.float32, device=xt.device)
-        return q, s, s.view((blocks,) + xt.shape[:-1]).movedim(0, -1)
-
-    def rmsnorm_fwd_fp8(self, x, r, w, eps):
-        lib = _native.load()
-        (xt, rows, ldx), C = x, w.numel()
-        q, s, scale = self._fp8_rows(xt, rows, C)
-        h = torch.empty(xt.shape, dtype=xt.dtype, device=xt.device) if r is not None else None
-        with _guard(xt):
-            rc = lib.dsw_rmsnorm_fwd_fp8(xt.data_ptr(), ldx, None if r is None else r[0].data_ptr(), 0 if r is None else r[2],
-                                         w.data_ptr(), q.data_ptr(), s.data_ptr(), rows, _ptr(h), rows, C, eps,
-                                         _DTYPES[xt.dtype], _stream(xt))
-        _native.check(rc, "dsw_rmsnorm_fwd_fp8")
-        return q, scale, h
-
-    def quant_fp8(self, x, C):
-        lib = _native.load()
-        xt, rows, ldx = x
-        q, s, scale = self._fp8_rows(xt, rows, C)
-        with _guard(xt):
-            rc = lib.dsw_quant_fp8(xt.data_ptr(), ldx, q.data_ptr(), s.data_ptr(), rows, rows, C, _DTYPES[xt.dtype], _stream(xt))
-        _native.check(rc, "dsw_quant_fp8")
-        return q, scale
-
-    def quant_fp8_weight(self, w):
-        lib = _native.load()
-        fin, fout = w.shape
-        q = torch.empty((fout, fin), dtype=torch.float8_e4m3fn, device=w.device)
-        s = torch.empty((_fp8_blocks(fout), _fp8_blocks(fin)), dtype=torch.float32, device=w.device)
-        with _guard(w):
-            rc = lib.dsw_quant_fp8_weight(w.data_ptr(), w.stride(0), w.stride(1), q.data_ptr(), s.data_ptr(), fin, fout,
-                                          _DTYPES[w.dtype], _stream(w))
-        _native.check(rc, "dsw_quant_fp8_weight")
-        return q, s
-
-    def fp8_mix(self, x, xs, wq, ws, bias, dtype):
-        lib = _native.load()
-        (xt, rows, ldx), (st, s_row, s_blk), (n, k) = x, xs, wq.shape
-        y = torch.empty(xt.shape[:-1] + (n,), dtype=dtype, device=xt.device)
-        with _guard(xt):
-            nb = int(lib.dsw_fp8_mix_workspace_bytes(rows, n, k))
-            if nb < 0:
-                _native.check(nb, "dsw_fp8_mix_workspace_bytes")
-            work = torch.empty((nb,), dtype=torch.uint8, device=xt.device) if nb else None
-            rc = lib.dsw_fp8_mix(xt.data_ptr(), ldx, st.data_ptr(), s_row, s_blk, wq.data_ptr(), wq.stride(0), ws.data_ptr(),
-                                 _ptr(bias), y.data_ptr(), rows, n, k, _DTYPES[dtype], _ptr(work), nb, _stream(xt))
-        _native.check(rc, "dsw_fp8_mix")
-        return y
-
-    def grad_norm_clip(self, grads, outs, norm_type, max_norm):
-        """``grads`` / ``outs`` (or None): dense tensors on one device, each pair of one shape, type and memory order."""
-        lib = _native.load()
-        dev = grads[0].device
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        ws = torch.empty((int(lib.dsw_grad_norm_workspace_bytes()),), dtype=torch.uint8, device=dev)
-        bf16 = torch.bfloat16
-        g = array.array("Q", [t.data_ptr() for t in grads])
-        o = g if outs is grads else None if outs is None else array.array("Q", [t.data_ptr() for t in outs])
-        sizes = array.array("q", [t.numel() for t in grads])
-        types = array.array("i", [1 if t.dtype is bf16 else 0 for t in grads])
-        with _guard(norm):
-            rc = lib.dsw_grad_norm_clip(len(grads), g.buffer_info()[0], None if o is None else o.buffer_info()[0],
-                                        sizes.buffer_info()[0], types.buffer_info()[0], norm_type, max_norm, norm.data_ptr(),
-                                        ws.data_ptr(), ws.numel(), _stream(norm))
-        _native.check(rc, "dsw_grad_norm_clip")
-        return norm
 
 
 _HIP = _HipBackend()
@@ -1385,132 +1256,9 @@ def cheb_basis(op: CsrOperator, x: torch.Tensor, K: int) -> torch.Tensor:
 
 
 # ----------------------------------------------------------------------------------------------
-# Row norm (training and 8-bit serving), 8-bit channel mix
+# Row norm (training and 8-bit serving), 8-bit channel mix, gradient norm and clipping: arguments are checked and backward
+# passes recorded by csrc/dsw_torch.cpp, which calls the same C entries (these operators take a few us on the card)
 # ----------------------------------------------------------------------------------------------
-FP8_BLOCK = 128        # channels per scale
-
-
-def _fp8_blocks(channels: int) -> int:
-    return -(-channels // FP8_BLOCK)
-
-
-def _as_rows(t: torch.Tensor, any_last: bool = False):
-    """``(t, rows, stride)``: ``t [..., C]`` as rows of C neighbouring elements, `stride` elements apart (channel slices of
-    wider tensors stay views; any other layout is copied).  ``any_last``: the last axis may have any stride of its own."""
-    C = t.shape[-1]
-    rows = t.numel() // C if C else 0
-    if t.is_contiguous():
-        return t, rows, C
-    sizes, strides = t.shape, t.stride()
-    ok = any_last or C == 1 or strides[-1] == 1
-    step = want = None
-    for size, st in zip(reversed(sizes[:-1]), reversed(strides[:-1])):
-        if size == 1:
-            continue
-        if step is None:
-            step = st
-        elif st != want:
-            ok = False
-        want = st * size
-    step = C if step is None else step
-    if not any_last and step < C:
-        ok = False                    # rows that overlap (a broadcast input)
-    if not ok or rows == 0:
-        t = t.contiguous()
-        step = C
-    return t, rows, step
-
-
-def _one_device(*tensors):
-    dev = tensors[0].device
-    for t in tensors[1:]:
-        if t is not None and t.device != dev:
-            raise ValueError(f"dsw: tensors on {dev} and {t.device} in one call")
-
-
-def _check_norm(x, weight, residual, eps):
-    if x.dim() < 1 or weight.dim() != 1 or x.shape[-1] != weight.shape[0] or x.shape[-1] == 0:
-        raise ValueError("expected x [..., C] and weight [C] with C >= 1")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError("expected a residual of the shape of x")
-    if not (eps >= 0.0 and math.isfinite(eps)):
-        raise ValueError("eps must be a finite number >= 0")
-    _check_dtype(x, weight, residual)
-    _one_device(x, weight, residual)
-
-
-# A leaf has ONE gradient accumulator, which belongs to the stream it was created on and lives as long as any graph over the
-# leaf.  A backward pass that is captured while such a graph of another stream is alive would hand the gradient to that other
-# stream, which then waits for the capture without ever joining it: ending the capture kills the process.  The accumulators
-# that a call meets are marked with the stream of the first one, and a captured backward pass refuses marks of another stream.
-_ACC_STREAM = "dsw_stream"
-
-
-def _mark_leaves(out, stream):
-    node = out.grad_fn
-    if node is not None:
-        for fn, _ in node.next_functions:
-            if hasattr(fn, "variable"):
-                fn.metadata.setdefault(_ACC_STREAM, stream)
-    return out
-
-
-def _refuse_foreign_leaves(ctx, t):
-    if not (t.is_cuda and torch.cuda.is_current_stream_capturing()):
-        return
-    stream = _stream(t)
-    for fn, _ in ctx.next_functions:
-        if hasattr(fn, "variable") and fn.metadata.get(_ACC_STREAM, stream) != stream:
-            raise RuntimeError("dsw: a backward pass is being captured while an earlier graph over the same leaf (shape %s) is alive "
-                               "on another stream; drop that graph (its outputs, its loss) before the capture" % (tuple(fn.variable.shape),))
-
-
-class _RmsNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, weight, eps):
-        be = _backend_for(x)
-        ctx.set_materialize_grads(False)
-        need = any(ctx.needs_input_grad[:3])
-        w = weight.contiguous()
-        rows = _as_rows(x)
-        y, h, rstd = be.rmsnorm_fwd(rows, None if residual is None else _as_rows(residual), w, eps, need)
-        if need:
-            # with a residual the stored stream h is read again by backward (it is alive anyway: the next block's input)
-            ctx.save_for_backward(rows[0] if residual is None else h, w, rstd)
-            ctx.be = be
-        return y if residual is None else (y, h)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dh=None):
-        h, w, rstd = ctx.saved_tensors
-        _refuse_foreign_leaves(ctx, h)
-        need_x, need_r, need_w = ctx.needs_input_grad[:3]
-        if dy is None:                       # nothing behind y: the stream's own gradient passes through
-            return (dh if need_x else None, dh if need_r else None, torch.zeros_like(w) if need_w else None, None)
-        dx, dw = ctx.be.rmsnorm_bwd(dy.contiguous(), None if dh is None else dh.contiguous(), _as_rows(h), w, rstd,
-                                    need_x or need_r, need_w)
-        return (dx if need_x else None, dx if need_r else None, dw, None)
-
-
-def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
-    """``y = x * (mean(x^2) + eps)^(-1/2) * weight`` over the last axis; ``x [..., C]`` fp32 or bf16 (a channel slice of a
-    wider tensor is read in place), ``weight [C]`` of the same type.  Sums in fp32; differentiable once."""
-    eps = float(eps)
-    _check_norm(x, weight, None, eps)
-    y = _RmsNormFn.apply(x, None, weight, eps)
-    return _mark_leaves(y, _stream(x)) if y.grad_fn is not None and y.is_cuda else y
-
-
-def rms_norm_residual(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6):
-    """``(rms_norm(h), h)`` with ``h = x + residual``, in one pass: ``h`` is the stream that the next residual addition
-    takes, the norm is taken of the unrounded sum.  Backward returns ONE tensor as the gradient of both addends."""
-    eps = float(eps)
-    _check_norm(x, weight, residual, eps)
-    y, h = _RmsNormFn.apply(x, residual, weight, eps)
-    return (_mark_leaves(y, _stream(x)) if y.grad_fn is not None and y.is_cuda else y), h
-
-
 class Fp8Rows(NamedTuple):
     """Rows in 8 bits: ``q [..., C]`` (float8_e4m3fn) stands for ``q * scale`` with one fp32 scale per row and 128 channels
     (``scale [..., ceil(C / 128)]``; the functions here lay the rows of one block next to each other in memory)."""
@@ -1527,119 +1275,59 @@ class Fp8Weight(NamedTuple):
     scale: torch.Tensor
 
 
-def _no_backward(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"dsw: {what} is a serving path without a backward pass; call it under torch.no_grad()")
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
+    """``y = x * (mean(x^2) + eps)^(-1/2) * weight`` over the last axis; ``x [..., C]`` fp32 or bf16 (a channel slice of a
+    wider tensor is read in place), ``weight [C]`` of the same type.  Sums in fp32; differentiable once."""
+    return _native.ops().rms_norm(x, weight, eps)
+
+
+def rms_norm_residual(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6):
+    """``(rms_norm(h), h)`` with ``h = x + residual``, in one pass: ``h`` is the stream that the next residual addition
+    takes, the norm is taken of the unrounded sum.  Backward returns ONE tensor as the gradient of both addends.  A backward
+    pass that is captured into a graph while an earlier graph over the same leaf lives on another stream is refused."""
+    return _native.ops().rms_norm_residual(x, residual, weight, eps)
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor = None, eps: float = 1e-6):
     """``(Fp8Rows of rms_norm(x (+ residual)), h)``: the norm with its output in e4m3, a scale per row and 128 channels, in the
     same pass; ``h`` is None without a residual.  Serving only (no backward)."""
-    eps = float(eps)
-    _check_norm(x, weight, residual, eps)
-    _no_backward("rms_norm_fp8", x, weight, residual)
-    be = _backend_for(x)
-    q, scale, h = be.rmsnorm_fwd_fp8(_as_rows(x), None if residual is None else _as_rows(residual), weight.contiguous(), eps)
+    q, scale, h = _native.ops().rms_norm_fp8(x, weight, residual, eps)
     return Fp8Rows(q, scale), h
 
 
 def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
-    """``x [..., C]`` (fp32 or bf16) in e4m3 with a scale per row and 128 channels: ``max|block| / 448``, not below 2^-126."""
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError("expected x [..., C] with C >= 1")
-    _check_dtype(x)
-    _no_backward("quantize_fp8", x)
-    return Fp8Rows(*_backend_for(x).quant_fp8(_as_rows(x), x.shape[-1]))
+    """``x [..., C]`` (fp32 or bf16) in e4m3 with a scale per row and 128 channels: ``max|block| / 448``, not below 2^-126.  A NaN
+    makes its block's scale a NaN."""
+    return Fp8Rows(*_native.ops().quantize_fp8(x))
 
 
 def quantize_fp8_weight(weight: torch.Tensor) -> Fp8Weight:
     """``weight [Fin, Fout]`` (as :func:`dense_mix` takes it, any strides) as an :class:`Fp8Weight`; once per model."""
-    if weight.dim() != 2 or weight.numel() == 0:
-        raise ValueError("expected weight [Fin, Fout]")
-    _check_dtype(weight)
-    _no_backward("quantize_fp8_weight", weight)
-    return Fp8Weight(*_backend_for(weight).quant_fp8_weight(weight))
+    return Fp8Weight(*_native.ops().quantize_fp8_weight(weight))
 
 
 def dense_mix_fp8(x, weight: Fp8Weight, bias: torch.Tensor = None, dtype: torch.dtype = None) -> torch.Tensor:
     """``y = x @ weight (+ bias)`` over the last axis on the 8-bit matrix cores: every block of 128 channels is summed in fp32,
     scaled by its two scales and added in fp32 (a bf16 output uses 8-bit matrix instructions, which drop what lies 13 bits below
-    the largest of 8 neighbouring products; an fp32 output exact products).  ``x``: :class:`Fp8Rows`, or an fp32 / bf16 tensor (quantised first);
-    ``dtype``: the output's (default: the tensor's, bfloat16 for rows), which ``bias [Fout]`` shares.  Serving only."""
+    the largest of 8 neighbouring products; an fp32 output exact products).  ``x``: :class:`Fp8Rows`, or an fp32 / bf16 tensor
+    (quantised first); ``dtype``: the output's (default: the tensor's, bfloat16 for rows), which ``bias [Fout]`` shares.  Serving
+    only (no backward)."""
     if not isinstance(weight, Fp8Weight):
         raise TypeError("dsw: weight must be an Fp8Weight (quantize_fp8_weight)")
     if isinstance(x, torch.Tensor):
         if x.dim() < 1 or x.shape[-1] != weight.q.shape[-1]:
             raise ValueError("expected x [..., Fin] and weight.q [Fout, Fin]")
-        _no_backward("dense_mix_fp8", x, bias)
         dtype = x.dtype if dtype is None else dtype
         x = quantize_fp8(x)
     elif not isinstance(x, Fp8Rows):
         raise TypeError("dsw: x must be a tensor or Fp8Rows")
-    dtype = torch.bfloat16 if dtype is None else dtype
-    q, wq = x.q, weight.q
-    if q.dtype != torch.float8_e4m3fn or wq.dtype != torch.float8_e4m3fn:
-        raise TypeError("dsw: 8-bit operands are float8_e4m3fn")
-    if x.scale.dtype != torch.float32 or weight.scale.dtype != torch.float32:
-        raise TypeError("dsw: scales are float32")
-    if dtype not in _DTYPES:
-        raise TypeError(f"dsw: unsupported dtype {dtype}; the HIP path implements float32 and bfloat16")
-    if q.dim() < 1 or wq.dim() != 2 or q.shape[-1] != wq.shape[1] or wq.numel() == 0:
-        raise ValueError("expected x.q [..., Fin] and weight.q [Fout, Fin]")
-    n, k = wq.shape
-    if tuple(x.scale.shape) != tuple(q.shape[:-1]) + (_fp8_blocks(k),):
-        raise ValueError("expected x.scale [..., ceil(Fin / 128)]")
-    if tuple(weight.scale.shape) != (_fp8_blocks(n), _fp8_blocks(k)):
-        raise ValueError("expected weight.scale [ceil(Fout / 128), ceil(Fin / 128)]")
-    if bias is not None and (bias.dim() != 1 or bias.shape[0] != n):
-        raise ValueError("expected bias [Fout]")
-    if bias is not None and bias.dtype != dtype:
-        raise TypeError(f"dsw: mixed dtypes {dtype} vs {bias.dtype}")
-    _one_device(q, x.scale, wq, weight.scale, bias)
-    _no_backward("dense_mix_fp8", bias)
-    be = _backend_for(q)
-    if wq.stride(1) != 1 or not k <= wq.stride(0) < 1 << 24:
-        wq = wq.contiguous()
-    rows = _as_rows(q)
-    if rows[2] >= 1 << 24:
-        rows = _as_rows(q.contiguous())
-    st, _, s_row = _as_rows(x.scale, any_last=True)
-    return be.fp8_mix(rows, (st, s_row, st.stride(-1)), wq, weight.scale.contiguous(), None if bias is None else bias.contiguous(), dtype)
-
-
-# ----------------------------------------------------------------------------------------------
-# Gradient norm and clipping
-# ----------------------------------------------------------------------------------------------
-def _dense(t: torch.Tensor) -> bool:
-    """Covers consecutive elements of its storage, in some dimension order."""
-    if t.is_contiguous():
-        return True
-    from .parallel import _is_permuted_dense
-
-    return t.numel() == 0 or _is_permuted_dense(t)
-
-
-def _grad_list(tensors, norm_type):
-    grads = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    norm_type = float(norm_type)
-    if norm_type not in (1.0, 2.0, math.inf):
-        raise ValueError("norm_type must be 1, 2 or inf")
-    if not grads:
-        raise ValueError("expected at least one gradient tensor")
-    for dt in set(map(attrgetter("dtype"), grads)):
-        if dt not in _DTYPES:
-            raise TypeError(f"dsw: unsupported dtype {dt}; the HIP path implements float32 and bfloat16")
-    if len(set(map(attrgetter("device"), grads))) > 1:
-        raise ValueError("dsw: gradients on more than one device in one call")
-    return grads, norm_type
+    return _native.ops().dense_mix_fp8(x.q, x.scale, weight.q, weight.scale, bias, torch.bfloat16 if dtype is None else dtype)
 
 
 def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     """Norm (1, 2 or inf) of all ``tensors`` taken together (fp32 and bf16, mixed, any shapes), a 0-dim fp32 tensor on their
     device.  Two launches for up to 144 tensors (a flat bucket's views count as one); sums in 64 bits; capturable."""
-    grads, norm_type = _grad_list(tensors, norm_type)
-    be = _backend_for(grads[0])
-    return be.grad_norm_clip([t if _dense(t) else t.contiguous() for t in grads], None, norm_type, 0.0)
+    return _native.ops().grad_norm_clip([tensors] if isinstance(tensors, torch.Tensor) else list(tensors), None, norm_type, 0.0, False)
 
 
 def clip_grad_norm_(tensors, max_norm: float, norm_type: float = 2.0, out=None) -> torch.Tensor:
@@ -1647,25 +1335,7 @@ def clip_grad_norm_(tensors, max_norm: float, norm_type: float = 2.0, out=None) 
     device: nothing is read back).  In place, or into ``out`` (a tensor of the same shape and type for each).  A tensor listed
     twice, or one that overlaps another one of the call, is refused.  A norm that is not finite behaves as the formula does:
     an infinite one gives zeros (and NaN in its infinite places), a NaN gives NaN."""
-    grads, norm_type = _grad_list(tensors, norm_type)
-    max_norm = float(max_norm)
-    if not max_norm >= 0.0:
-        raise ValueError("max_norm must be >= 0")
-    be = _backend_for(grads[0])
-    outs = grads
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if out is not None:
-        grads = list(grads)
-        outs = [out] if isinstance(out, torch.Tensor) else list(out)
-        if len(outs) != len(grads):
-            raise ValueError("expected one `out` tensor for each gradient")
-        for g, o in zip(grads, outs):
-            if g.shape != o.shape or g.dtype != o.dtype or g.device != o.device:
-                raise ValueError("`out` must have the gradients' shapes, types and device")
-    for i, (g, o) in enumerate(zip(grads, outs)):
-        if g.is_contiguous() and o.is_contiguous():
-            continue
-        if not _dense(o):
-            raise ValueError("dsw: a clipped tensor must be dense (cover consecutive elements, in any dimension order)")
-        if g.stride() != o.stride():                # the kernels walk both in memory order
-            grads[i] = torch.empty_strided(o.shape, o.stride(), dtype=o.dtype, device=o.device).copy_(g)
-    return be.grad_norm_clip(grads, outs, norm_type, max_norm)
+        out = [out] if isinstance(out, torch.Tensor) else list(out)
+    return _native.ops().grad_norm_clip(tensors, out, norm_type, max_norm, True)

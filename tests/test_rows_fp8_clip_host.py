@@ -11,27 +11,8 @@ from dsw_amd import _native, functional as F
 F8 = torch.float8_e4m3fn
 
 
-class _Reached(Exception):
-    pass
-
-
-class _Stop:
-    """A backend that only says that the call was let through."""
-
-    name = "stop"
-
-    def __getattr__(self, name):
-        def reached(*a, **k):
-            raise _Reached(name)
-
-        return reached
-
-
-@pytest.fixture()
-def stop():
-    F.set_test_backend(_Stop())
-    yield
-    F.set_test_backend(None)
+# a call that passes every check of its arguments ends at the device of its tensors
+passed = lambda: pytest.raises(RuntimeError, match="no CPU fallback")  # noqa: E731
 
 
 def test_cpu_tensors_are_refused():
@@ -44,7 +25,7 @@ def test_cpu_tensors_are_refused():
             call()
 
 
-def test_norm_refusals(stop):
+def test_norm_refusals():
     x, w = torch.randn(4, 8), torch.ones(8)
     with pytest.raises(ValueError):
         F.rms_norm(x, torch.ones(7))
@@ -69,19 +50,19 @@ def test_norm_refusals(stop):
         F.quantize_fp8(x.half())
     with pytest.raises(RuntimeError, match="no_grad"):
         F.rms_norm_fp8(x, torch.nn.Parameter(w))
-    with pytest.raises(_Reached):
+    with passed():
         with torch.no_grad():
             F.rms_norm_fp8(x, torch.nn.Parameter(w))
-    with pytest.raises(_Reached):
+    with passed():
         F.rms_norm_residual(x, x, w)
 
 
-def test_product_refusals(stop):
+def test_product_refusals():
     rows = F.Fp8Rows(torch.zeros(4, 300, dtype=F8), torch.ones(4, 3))
     weight = F.Fp8Weight(torch.zeros(130, 300, dtype=F8), torch.ones(2, 3))
-    with pytest.raises(_Reached):
+    with passed():
         F.dense_mix_fp8(rows, weight)
-    with pytest.raises(_Reached):
+    with passed():
         F.dense_mix_fp8(rows, weight, torch.zeros(130, dtype=torch.bfloat16))
     with pytest.raises(TypeError):
         F.dense_mix_fp8(rows, weight.q)
@@ -108,9 +89,9 @@ def test_product_refusals(stop):
         F.dense_mix_fp8(torch.randn(4, 300, requires_grad=True), weight)
 
 
-def test_clip_refusals(stop):
+def test_clip_refusals():
     g = [torch.randn(5), torch.randn(2, 3)]
-    with pytest.raises(_Reached):
+    with passed():
         F.clip_grad_norm_(g, 1.0)
     with pytest.raises(ValueError):
         F.clip_grad_norm_([], 1.0)
@@ -188,14 +169,15 @@ def test_clip_entry_refuses_overlap_and_bad_arguments():
 
 def test_rows_of_views():
     """(rows, stride) of the layouts the row kernels read in place, and the copies of the others."""
+    as_rows = _native.ops().as_rows
     t = torch.arange(2 * 6 * 40, dtype=torch.float32).view(2, 6, 40)
     for view, rows, step in ((t, 12, 40), (t[..., 8:24], 12, 40), (t[1], 6, 40), (t[0, 0], 1, 40), (t[:, :1], 2, 240), (t[:1, 2:5, :7], 3, 40)):
-        got = F._as_rows(view)
+        got = as_rows(view, False)
         assert got[0].data_ptr() == view.data_ptr() and got[1] == rows and (rows == 1 or got[2] == step), (view.shape, got[1:])
     for view in (t[:, 1:5, :8], t.transpose(1, 2), t[..., ::2], t[:1, :1].expand(2, 6, 40), t.flip(-1)):
-        got, rows, step = F._as_rows(view)
+        got, rows, step = as_rows(view, False)
         assert got.is_contiguous() and step == view.shape[-1] and torch.equal(got, view)
     scale = torch.empty(3, 12).view(3, 2, 6).movedim(0, -1)
-    got, rows, step = F._as_rows(scale, any_last=True)
-    assert got is scale and (rows, step, got.stride(-1)) == (12, 1, 12)
-    assert F._as_rows(torch.ones(1, 3).expand(12, 3), any_last=True)[2] == 0
+    got, rows, step = as_rows(scale, True)
+    assert got.data_ptr() == scale.data_ptr() and got.stride() == scale.stride() and (rows, step, got.stride(-1)) == (12, 1, 12)
+    assert as_rows(torch.ones(1, 3).expand(12, 3), True)[2] == 0
