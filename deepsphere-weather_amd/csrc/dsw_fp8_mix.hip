@@ -61,13 +61,24 @@ static __device__ __forceinline__ f32x4 block_product(const Frag<WIDE>& a, const
     }
 }
 
-// 16 bytes k .. k + 15 of a row of K bytes; what lies behind the row is zero
+static __device__ __forceinline__ u32x4 chunk(const uint8_t* p) { return reinterpret_cast<const Any16*>(p)->v; }
+// 16 bytes k .. k + 15 of a row of K bytes; what lies behind the row is zero.  A chunk that the row ends in is read as the row's
+// last 16 bytes and shifted down (one load; byte by byte it would be a chain of up to 15).
 static __device__ __forceinline__ u32x4 row_chunk(const uint8_t* row, int k, int K) {
     u32x4 t = {0u, 0u, 0u, 0u};
     if (k + 16 <= K) {
-        t = reinterpret_cast<const Any16*>(row + k)->v;
+        t = chunk(row + k);
     } else if (k < K) {
-        for (int j = 0; j < K - k; ++j) t[j >> 2] |= (uint32_t)row[k + j] << (8 * (j & 3));
+        if (K >= 16) {
+            const u32x4 e = chunk(row + K - 16);
+            uint64_t lo = (uint64_t)e[1] << 32 | e[0], hi = (uint64_t)e[3] << 32 | e[2];
+            const int cut = 8 * (k + 16 - K);                   // 8 .. 120 bits
+            if (cut >= 64) { lo = hi >> (cut - 64); hi = 0; }
+            else { lo = lo >> cut | hi << (64 - cut); hi >>= cut; }
+            t = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+        } else {
+            for (int j = 0; j < K - k; ++j) t[j >> 2] |= (uint32_t)row[k + j] << (8 * (j & 3));
+        }
     }
     return t;
 }
@@ -147,8 +158,8 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
         } else {
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
-                const uint8_t* p = (i < BN / 8 / WAVES ? wbase : xbase) + off[i] + (long)b * 128;
-                held[i] = row_chunk(p, 0, P.K - b * 128 - piece_chunk(i) * 16);
+                const int at = piece_chunk(i) * 16;
+                held[i] = row_chunk((i < BN / 8 / WAVES ? wbase : xbase) + off[i] - at, b * 128 + at, P.K);
             }
         }
     };
@@ -204,16 +215,29 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
             const int r = BN + wm + 16 * j + r16, f = r16 & 7;
             fx[j] = make_frag<WIDE>(base[r * 8 + (g ^ f)], base[r * 8 + ((g + 4) ^ f)]);
         }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
+        // products of step t are added while those of step t + 1 are on the matrix cores: a product takes 32 clocks, its four
+        // additions 16, and the vector pipe reads a result no sooner than its matrix instruction has ended
+        auto weight_frag = [&](int t) {
             const int r = wn + 4 * NT * (r16 >> 2) + 4 * t + (r16 & 3), f = w_place<NT>(r);
-            const Frag<WIDE> fw = make_frag<WIDE>(base[r * 8 + (g ^ f)], base[r * 8 + ((g + 4) ^ f)]);
+            return make_frag<WIDE>(base[r * 8 + (g ^ f)], base[r * 8 + ((g + 4) ^ f)]);
+        };
+        Frag<WIDE> fw = weight_frag(0);
+        f32x4 p[MT];
+#pragma unroll
+        for (int t = 0; t <= NT; ++t) {
+            Frag<WIDE> next = fw;
+            if (t + 1 < NT) next = weight_frag(t + 1);
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
-                const f32x4 p = block_product<WIDE>(fw, fx[j]);
+                f32x4 q = p[j];
+                if (t < NT) p[j] = block_product<WIDE>(fw, fx[j]);
+                if (t > 0) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) acc[t][j][k] = fmaf(p[k], s[j], acc[t][j][k]);
+                    for (int k = 0; k < 4; ++k) acc[t - 1][j][k] = fmaf(q[k], s[j], acc[t - 1][j][k]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
+            fw = next;
         }
         if (b + 1 < P.KB) store_held(stage ^ 1);
     }
@@ -261,9 +285,10 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
 
 // ---- few rows: 16 outputs n x 16 MT rows m per workgroup; the waves share the blocks of K ------------------------------------
 // Bound by reading the weights: every wave reads the 16 weight rows of its blocks straight into registers (16 bytes per lane and
-// load, any alignment), the partial sums of the waves are joined in wave order through LDS.
+// load, any alignment), U blocks at a time so that their loads are in flight together; the partial sums of the waves are joined in
+// wave order through LDS.
 constexpr int FEW_WAVES = 8;
-template <int MT, bool BF16>
+template <int MT, int U, bool BF16>
 __global__ __launch_bounds__(64 * FEW_WAVES) void fp8_mix_few_kernel(const MixArgs P) {
     constexpr bool WIDE = !BF16;
     __shared__ float part[FEW_WAVES][MT * 4][64];
@@ -283,17 +308,51 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void fp8_mix_few_kernel(const MixAr
     f32x4 acc[MT];
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int b = wave; b < P.KB; b += FEW_WAVES) {
-        const int k = b * 128 + g * 16;
-        const Frag<WIDE> fw = make_frag<WIDE>(row_chunk(w, k, P.K), row_chunk(w, k + 64, P.K));
+    auto add = [&](const u32x4 (&wc)[2], const u32x4 (&xc)[MT][2], float sw, const float (&sx)[MT]) {
+        const Frag<WIDE> fw = make_frag<WIDE>(wc[0], wc[1]);
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-            const Frag<WIDE> fx = make_frag<WIDE>(row_chunk(x[j], k, P.K), row_chunk(x[j], k + 64, P.K));
-            const float s = ws[b] * xs[j][(long)b * P.xs_blk];
-            const f32x4 p = block_product<WIDE>(fw, fx);
+            const f32x4 p = block_product<WIDE>(fw, make_frag<WIDE>(xc[j][0], xc[j][1]));
+            const float s = sw * sx[j];
 #pragma unroll
             for (int q = 0; q < 4; ++q) acc[j][q] = fmaf(p[q], s, acc[j][q]);
         }
+    };
+    const int whole = P.K >> 7;
+    for (int b0 = wave; b0 < whole; b0 += FEW_WAVES * U) {
+        u32x4 wc[U][2], xc[U][MT][2];
+        float sw[U], sx[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int b = b0 + u * FEW_WAVES;
+            if (b < whole) {                           // (uniform)
+                const long k = (long)b * 128 + g * 16;
+                wc[u][0] = chunk(w + k);
+                wc[u][1] = chunk(w + k + 64);
+                sw[u] = ws[b];
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    xc[u][j][0] = chunk(x[j] + k);
+                    xc[u][j][1] = chunk(x[j] + k + 64);
+                    sx[u][j] = xs[j][(long)b * P.xs_blk];
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (b0 + u * FEW_WAVES < whole) add(wc[u], xc[u], sw[u], sx[u]);
+    }
+    if (whole < P.KB && wave == whole % FEW_WAVES) {   // the short last block, by the wave whose turn it is
+        const int k = whole * 128 + g * 16;
+        u32x4 wc[2] = {row_chunk(w, k, P.K), row_chunk(w, k + 64, P.K)}, xc[MT][2];
+        float sx[MT];
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            xc[j][0] = row_chunk(x[j], k, P.K);
+            xc[j][1] = row_chunk(x[j], k + 64, P.K);
+            sx[j] = xs[j][(long)whole * P.xs_blk];
+        }
+        add(wc, xc, ws[whole], sx);
     }
 #pragma unroll
     for (int j = 0; j < MT; ++j)
@@ -329,10 +388,11 @@ static int launch_tile(const MixArgs& a, hipStream_t s) {
 template <bool BF16>
 static int launch_few(const MixArgs& a, hipStream_t s) {
     const unsigned gn = (unsigned)((a.N + 15) / 16);
-#define FEW(MT_) DSW_LAUNCH((fp8_mix_few_kernel<MT_, BF16>), dim3(gn, (unsigned)((a.M + 16 * MT_ - 1) / (16 * MT_))), dim3(64 * FEW_WAVES), 0, s, a)
-    if (a.M <= 16) FEW(1);
-    else if (a.M <= 32) FEW(2);
-    else FEW(4);
+#define FEW(MT_, U_) DSW_LAUNCH((fp8_mix_few_kernel<MT_, U_, BF16>), dim3(gn, (unsigned)((a.M + 16 * MT_ - 1) / (16 * MT_))), dim3(64 * FEW_WAVES), 0, s, a)
+    if (a.M <= 16) FEW(1, 4);
+    else if (a.M <= 32) FEW(2, 2);
+    else if (a.M <= 48) FEW(3, 2);
+    else FEW(4, 2);
 #undef FEW
     return dsw_check_launch();
 }
