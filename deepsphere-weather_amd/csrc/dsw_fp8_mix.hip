@@ -94,162 +94,61 @@ static __device__ __forceinline__ void store_out(void* p, long i, float v) {
     else static_cast<float*>(p)[i] = v;
 }
 
-// One lane's 16 bytes global memory -> LDS (lane l of the wave writes LDS byte `lds` + 16 l); waited for by hand (vmcnt).
+// Global memory -> LDS without registers: lane l's 16 (4) bytes land at LDS byte `lds` + 16 l (4 l).  The compiler does not count
+// these loads: they are waited for by hand.
 static __device__ __forceinline__ void load_to_lds(const uint8_t* base, uint32_t off, uint32_t lds) {
     uint32_t m0;
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
                  : "=&s"(m0) : "v"(off), "s"(base), "s"(lds) : "memory");
 }
+static __device__ __forceinline__ void load_to_lds4(const float* at, uint32_t lds) {
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "v"(at), "s"(lds) : "memory");
+}
+static __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+static __device__ __forceinline__ uint32_t lds_byte(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
+// (uniform index: a scalar load, which the counts of vector loads do not see)
+static __device__ __forceinline__ float scalar_load(const float* p, int i) {
+    return reinterpret_cast<const __attribute__((address_space(4))) float*>(reinterpret_cast<uintptr_t>(p))[i];
+}
 
-// ---- many rows: tiles of (16 NT WN) outputs n x (16 MT WM) rows m per workgroup of WN x WM waves -----------------------------
-// Operands travel through LDS, one scale block (128 bytes of every row) per step, two stages: while a block is multiplied the
-// next one is on its way.  Row r of a stage is 128 bytes, its 16-byte chunk c sits at place c ^ f(r), so that the 16 rows a
-// fragment reads spread over the banks.  Which n a row of the matrix instruction stands for is free: row r of tile t of a wave is
-// n = 4 NT (r / 4) + 4 t + r % 4, so that a lane ends with 4 NT neighbouring outputs of one row m and stores whole 16 bytes.
-// DMA: 16-byte aligned rows of whole 16-byte chunks go to LDS directly; otherwise through registers.
+// ---- many rows: tiles of 16 NT WN outputs n x 16 MT WM rows m per workgroup of WN x WM waves ---------------------------------
+// Operands travel through LDS, one scale block (128 bytes of every row) per stage.  Row r of a stage is 128 bytes, its 16-byte
+// chunk c sits at place c ^ f(r), so that the 16 rows a fragment reads spread over the banks.  Which n a row of the matrix
+// instruction stands for is free: row r of tile t of a wave is n = 4 NT (r / 4) + 4 t + r % 4, so that a lane ends with 4 NT
+// neighbouring outputs of one row m and stores whole 16 bytes.
 template <int NT>
 static __device__ __forceinline__ int w_place(int row) { return (row & 3) | (((row / (4 * NT)) & 1) << 2); }
 
-template <int NT, int MT, int WN, int WM, bool BF16, bool DMA>
-__global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArgs P, const int tiles_n, const int tiles_m) {
-    constexpr bool WIDE = !BF16;
-    constexpr int WAVES = WN * WM, BN = 16 * NT * WN, BM = 16 * MT * WM, ROWS = BN + BM, PIECES = ROWS / 8 / WAVES;
-    static_assert(ROWS % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "a wave's pieces lie in one operand each");
-    static_assert(128 % (16 * NT) == 0, "a wave's outputs share a row of weight scales");
-    extern __shared__ u32x4 lds[];                     // [2][ROWS][8]
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // tiles: each of the 8 dies takes a contiguous run of them (blocks go round the dies), 8 row tiles deep
+// tiles of a grid: each of the 8 dies takes a contiguous run of them (blocks go round the dies), 8 row tiles deep, so that the
+// tiles that one L2 serves at a time share rows and weights
+static __device__ __forceinline__ bool tile_of(int tiles_n, int tiles_m, int& tn, int& tm) {
     const int T = tiles_n * tiles_m, per = (T + 7) >> 3;
-    const int t_id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if (t_id >= T) return;
-    const int deep = 8, band = t_id / (deep * tiles_n), in = t_id - band * deep * tiles_n;
+    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (id >= T) return false;
+    const int deep = 8, band = id / (deep * tiles_n), in = id - band * deep * tiles_n;
     const int high = tiles_m - band * deep < deep ? tiles_m - band * deep : deep;
-    const int n0 = (in / high) * BN, m0 = (band * deep + in % high) * BM;
-    const int wn = (wave % WN) * 16 * NT, wm = (wave / WN) * 16 * MT;
-    const int r16 = lane & 15, g = lane >> 4;
+    tn = in / high;
+    tm = band * deep + in % high;
+    return true;
+}
 
-    // this lane's share of a stage: PIECES chunks, the first BN / 8 pieces are weight rows
-    uint32_t off[PIECES];
-    const uint8_t* const wbase = P.W + (long)n0 * P.ldw;
-    const uint8_t* const xbase = P.X + (long)m0 * P.ldx;
-    auto piece_row = [&](int i) { return (wave + i * WAVES) * 8 + (lane >> 3); };
-    auto piece_chunk = [&](int i) {
-        const int row = piece_row(i);
-        return row < BN ? (lane & 7) ^ w_place<NT>(row) : (lane & 7) ^ ((row - BN) & 7);
-    };
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-        const int row = piece_row(i);
-        if (row < BN) off[i] = (uint32_t)((n0 + row < P.N ? row : P.N - 1 - n0) * P.ldw) + piece_chunk(i) * 16;
-        else off[i] = (uint32_t)((m0 + row - BN < P.M ? row - BN : P.M - 1 - m0) * P.ldx) + piece_chunk(i) * 16;
-    }
-    const int whole = P.K >> 7, tail = P.K & 127;      // whole blocks, bytes of the last one
-    u32x4 held[DMA ? 1 : PIECES];
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-    auto fetch = [&](int b, int stage) {
-        if constexpr (DMA) {
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                const bool w = i < BN / 8 / WAVES;
-                uint32_t o = off[i];
-                if (b == whole) { const int c = piece_chunk(i); o = c * 16 < tail ? o : o - c * 16; }    // (chunks behind the row: cleared below)
-                load_to_lds((w ? wbase : xbase) + (long)b * 128, o, lds0 + (uint32_t)((stage * ROWS + (wave + i * WAVES) * 8) * 128));
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                const int at = piece_chunk(i) * 16;
-                held[i] = row_chunk((i < BN / 8 / WAVES ? wbase : xbase) + off[i] - at, b * 128 + at, P.K);
-            }
-        }
-    };
-    auto store_held = [&](int stage) {
-        if constexpr (!DMA) {
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i) lds[(stage * ROWS + piece_row(i)) * 8 + (lane & 7)] = held[i];
-        }
-    };
-
-    const float* xs[MT];
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-        const int m = m0 + wm + 16 * j + r16;
-        xs[j] = P.XS + (long)(m < P.M ? m : P.M - 1) * P.xs_row;
-    }
-    const int nb = (n0 + wn) >> 7, nb_last = (P.N - 1) >> 7;
-    const float* const ws = P.WS + (long)(nb < nb_last ? nb : nb_last) * P.KB;
-
-    f32x4 acc[NT][MT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float sx[MT], sw = ws[0];
-#pragma unroll
-    for (int j = 0; j < MT; ++j) sx[j] = xs[j][0];
-    fetch(0, 0);
-    store_held(0);
-    for (int b = 0; b < P.KB; ++b) {
-        const int stage = b & 1;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();                               // the block has landed; the other stage is no longer read
-        if (DMA && b == whole) {                       // the last block is short: clear what lies behind the rows
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i)
-                if (piece_chunk(i) * 16 >= tail) lds[(stage * ROWS + piece_row(i)) * 8 + (lane & 7)] = u32x4{0u, 0u, 0u, 0u};
-            __syncthreads();
-        }
-        float s[MT];
-#pragma unroll
-        for (int j = 0; j < MT; ++j) s[j] = sw * sx[j];
-        if (b + 1 < P.KB) {
-            sw = ws[b + 1];
-#pragma unroll
-            for (int j = 0; j < MT; ++j) sx[j] = xs[j][(long)(b + 1) * P.xs_blk];
-            fetch(b + 1, stage ^ 1);
-        }
-        const u32x4* const base = lds + stage * ROWS * 8;
-        Frag<WIDE> fx[MT];
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-            const int r = BN + wm + 16 * j + r16, f = r16 & 7;
-            fx[j] = make_frag<WIDE>(base[r * 8 + (g ^ f)], base[r * 8 + ((g + 4) ^ f)]);
-        }
-        // products of step t are added while those of step t + 1 are on the matrix cores: a product takes 32 clocks, its four
-        // additions 16, and the vector pipe reads a result no sooner than its matrix instruction has ended
-        auto weight_frag = [&](int t) {
-            const int r = wn + 4 * NT * (r16 >> 2) + 4 * t + (r16 & 3), f = w_place<NT>(r);
-            return make_frag<WIDE>(base[r * 8 + (g ^ f)], base[r * 8 + ((g + 4) ^ f)]);
-        };
-        Frag<WIDE> fw = weight_frag(0);
-        f32x4 p[MT];
-#pragma unroll
-        for (int t = 0; t <= NT; ++t) {
-            Frag<WIDE> next = fw;
-            if (t + 1 < NT) next = weight_frag(t + 1);
-#pragma unroll
-            for (int j = 0; j < MT; ++j) {
-                f32x4 q = p[j];
-                if (t < NT) p[j] = block_product<WIDE>(fw, fx[j]);
-                if (t > 0) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[t - 1][j][k] = fmaf(q[k], s[j], acc[t - 1][j][k]);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            fw = next;
-        }
-        if (b + 1 < P.KB) store_held(stage ^ 1);
-    }
-
-    const int n = n0 + wn + 4 * NT * g;
+// a wave's results: lane (r16, g) holds outputs n0 + 4 NT g .. + 4 NT - 1 of the rows m0 + 16 j + r16
+template <int NT, int MT, bool BF16>
+static __device__ __forceinline__ void store_tile(const MixArgs& P, const f32x4 (&acc)[NT][MT], int n0, int m0, int r16, int g) {
+    const int n = n0 + 4 * NT * g;
     float add[4 * NT];
 #pragma unroll
-    for (int k = 0; k < 4 * NT; ++k) add[k] = P.bias != nullptr && n + k < P.N ? load_out<BF16>(P.bias, n + k) : 0.f;
+    for (int k = 0; k < 4 * NT; ++k) add[k] = 0.f;
+    if (P.bias != nullptr) {
+#pragma unroll
+        for (int k = 0; k < 4 * NT; ++k) add[k] = n + k < P.N ? load_out<BF16>(P.bias, n + k) : 0.f;
+    }
     const bool vec = n + 4 * NT <= P.N && P.N % 8 == 0 && ((uintptr_t)P.Y & 15) == 0;
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
-        const int m = m0 + wm + 16 * j + r16;
+        const int m = m0 + 16 * j + r16;
         if (m >= P.M) continue;
         const long at = (long)m * P.N + n;
         if (vec) {
@@ -283,52 +182,287 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
     }
 }
 
-// ---- few rows: 16 outputs n x 16 MT rows m per workgroup; the waves share the blocks of K ------------------------------------
-// Bound by reading the weights: every wave reads the 16 weight rows of its blocks straight into registers (16 bytes per lane and
-// load, any alignment), U blocks at a time so that their loads are in flight together; the partial sums of the waves are joined in
-// wave order through LDS.
-constexpr int FEW_WAVES = 8;
-template <int MT, int U, bool BF16>
-__global__ __launch_bounds__(64 * FEW_WAVES) void fp8_mix_few_kernel(const MixArgs P) {
+// 16-byte aligned rows of whole 16-byte chunks: two stages in LDS, filled without registers.  One meeting per block, before its
+// last step t: by then every wave has read its last weights of the block, so its stage takes the loads of the block after next,
+// and the next block has landed (its loads had a whole block's time), so its first fragments are read while the last step's
+// products are computed.  The matrix cores thus wait neither for the barrier nor for the fragments behind it.
+// The products of one step are scaled and added while the next step's are computed: a 16x16x128 product takes 32 clocks, of which
+// the vector unit is free for 16, its four additions (measured: 4 additions a product cost 12 %, each further instruction 4
+// clocks) - so the loop's addresses are scalars and immediates.
+template <int NT, int MT, int WN, int WM, bool BF16>
+__global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArgs P, const int tiles_n, const int tiles_m) {
     constexpr bool WIDE = !BF16;
-    __shared__ float part[FEW_WAVES][MT * 4][64];
+    constexpr int WAVES = WN * WM, BN = 16 * NT * WN, BM = 16 * MT * WM, ROWS = BN + BM, PIECES = ROWS / 8 / WAVES;
+    constexpr int STAGE = ROWS * 8 + WAVES * 16;       // 16-byte units: the rows, then 64 row scales of each wave
+    static_assert(ROWS % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "a wave's pieces lie in one operand each");
+    static_assert(128 % (16 * NT) == 0, "a wave's outputs share a row of weight scales");
+    static_assert(MT <= 4 && NT >= 2 && NT % 2 == 0 && PIECES < (NT - 1) * MT, "every load is issued before the last step");
+    extern __shared__ u32x4 lds[];                     // [2][STAGE]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
+    int tn, tm;
+    if (!tile_of(tiles_n, tiles_m, tn, tm)) return;
+    const int n0 = tn * BN, m0 = tm * BM;
+    const int wn = (wave % WN) * 16 * NT, wm = (wave / WN) * 16 * MT;
     const int r16 = lane & 15, g = lane >> 4;
-    const uint8_t* const w = P.W + (long)(n0 + r16 < P.N ? n0 + r16 : P.N - 1) * P.ldw;
+
+    // this lane's share of a stage: PIECES chunks (the first BN / 8 pieces are weight rows) and one row scale
+    uint32_t off[PIECES];
+    auto piece_row = [&](int i) { return (wave + i * WAVES) * 8 + (lane >> 3); };
+    auto piece_chunk = [&](int i) {
+        const int row = piece_row(i);
+        return row < BN ? (lane & 7) ^ w_place<NT>(row) : (lane & 7) ^ ((row - BN) & 7);
+    };
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int row = piece_row(i);
+        if (row < BN) off[i] = (uint32_t)((n0 + row < P.N ? row : P.N - 1 - n0) * P.ldw) + piece_chunk(i) * 16;
+        else off[i] = (uint32_t)((m0 + row - BN < P.M ? row - BN : P.M - 1 - m0) * P.ldx) + piece_chunk(i) * 16;
+    }
+    const int ms = m0 + wm + (lane < 16 * MT ? lane : 0);
+    const float* xs = P.XS + (long)(ms < P.M ? ms : P.M - 1) * P.xs_row;      // of the next block to be fetched
+    const int nb = (n0 + wn) >> 7, nb_last = (P.N - 1) >> 7;
+    const float* const ws = P.WS + (long)(nb < nb_last ? nb : nb_last) * P.KB;
+    const uint8_t* wk = P.W + (long)n0 * P.ldw;                               // of the next block to be fetched
+    const uint8_t* xk = P.X + (long)m0 * P.ldx;
+    const uint32_t lds0 = lds_byte(lds);
+    const int whole = P.K >> 7, tail = P.K & 127;      // whole blocks, bytes of the last one
+    auto fetch_piece = [&](int i, uint32_t o, int stage) {
+        load_to_lds(i < BN / 8 / WAVES ? wk : xk, o, lds0 + (uint32_t)(stage * STAGE * 16 + (wave + i * WAVES) * 1024));
+    };
+    auto fetch_scales = [&](int stage) { load_to_lds4(xs, lds0 + (uint32_t)((stage * STAGE + ROWS * 8 + wave * 16) * 16)); };
+    // places of this lane's chunks g and g + 4 in a stage: of row tile 0 (128 apart per tile), of weight tile 0 (32 apart)
+    const int x_row = (BN + wm + r16) * 8, x_lo = x_row + (g ^ (r16 & 7)), x_hi = x_row + ((g + 4) ^ (r16 & 7));
+    const int w_r = wn + 4 * NT * (r16 >> 2) + (r16 & 3), w_f = w_place<NT>(w_r);
+    const int w_lo = w_r * 8 + (g ^ w_f), w_hi = w_r * 8 + ((g + 4) ^ w_f);
+    const int s_at = (ROWS * 8 + wave * 16) * 4 + r16;
+
+    f32x4 acc[NT][MT], p[MT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        p[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (whole > 0) {
+        auto advance = [&](bool on) { wk += on ? 128 : 0; xk += on ? 128 : 0; xs += on ? P.xs_blk : 0; };
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) fetch_piece(i, off[i], 0);
+        fetch_scales(0);
+        advance(whole > 1);
+        wait_loads();
+        __syncthreads();
+        Frag<WIDE> fx[MT], fw = make_frag<WIDE>(lds[w_lo], lds[w_hi]);
+        float s[MT], s_old[MT];
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            fx[j] = make_frag<WIDE>(lds[x_lo + 128 * j], lds[x_hi + 128 * j]);
+            s[j] = scalar_load(ws, 0) * reinterpret_cast<const float*>(lds)[s_at + 16 * j];
+            s_old[j] = 0.f;
+        }
+        // No branch in the loop (the additions have to stay between the products): behind the last block it fetches that block
+        // again, into the stage that nobody reads any more.
+        int stage = 0;
+        for (int b = 0; b < whole; ++b) {
+            const u32x4* const here = lds + stage * STAGE;
+            const u32x4* const there = lds + (stage ^ 1) * STAGE;
+            const float sw = scalar_load(ws, b + 1 < whole ? b + 1 : b);
+            float s_next[MT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                Frag<WIDE> next;
+                if (t + 1 < NT) {
+                    next = make_frag<WIDE>(here[w_lo + 32 * (t + 1)], here[w_hi + 32 * (t + 1)]);
+                } else {
+                    wait_loads();
+                    __syncthreads();
+                    next = make_frag<WIDE>(there[w_lo], there[w_hi]);
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) s_next[j] = sw * reinterpret_cast<const float*>(there)[s_at + 16 * j];
+                }
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    const f32x4 q = p[j];
+                    const float sq = t == 0 ? s_old[j] : s[j];
+                    p[j] = block_product<WIDE>(fw, fx[j]);
+                    if (t * MT + j < PIECES) fetch_piece(t * MT + j, off[t * MT + j], stage ^ 1);
+                    if (t * MT + j == PIECES) fetch_scales(stage ^ 1);
+                    if (t + 1 == NT) fx[j] = make_frag<WIDE>(there[x_lo + 128 * j], there[x_hi + 128 * j]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[(t + NT - 1) % NT][j][k] = fmaf(q[k], sq, acc[(t + NT - 1) % NT][j][k]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                fw = next;
+            }
+#pragma unroll
+            for (int j = 0; j < MT; ++j) { s_old[j] = s[j]; s[j] = s_next[j]; }
+            advance(b + 2 < whole);
+            stage ^= 1;
+        }
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[NT - 1][j][k] = fmaf(p[j][k], s_old[j], acc[NT - 1][j][k]);
+        if (tail) advance(true);
+        __syncthreads();
+    }
+    if (tail) {                                        // the short last block: its chunks behind the rows are cleared in LDS
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) { const int c = piece_chunk(i) * 16; fetch_piece(i, c < tail ? off[i] : off[i] - c, 0); }
+        fetch_scales(0);
+        wait_loads();
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+            if (piece_chunk(i) * 16 >= tail) lds[piece_row(i) * 8 + (lane & 7)] = u32x4{0u, 0u, 0u, 0u};
+        __syncthreads();
+        const float sw = scalar_load(ws, whole);
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            const Frag<WIDE> fx = make_frag<WIDE>(lds[x_lo + 128 * j], lds[x_hi + 128 * j]);
+            const float s = sw * reinterpret_cast<const float*>(lds)[s_at + 16 * j];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const f32x4 q = block_product<WIDE>(make_frag<WIDE>(lds[w_lo + 32 * t], lds[w_hi + 32 * t]), fx);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[t][j][k] = fmaf(q[k], s, acc[t][j][k]);
+            }
+        }
+    }
+    store_tile<NT, MT, BF16>(P, acc, n0 + wn, m0 + wm, r16, g);
+}
+
+// any alignment and strides: the same tiles, two stages, filled through registers
+template <int NT, int MT, int WN, int WM, bool BF16>
+__global__ __launch_bounds__(64 * WN * WM) void fp8_mix_any_kernel(const MixArgs P, const int tiles_n, const int tiles_m) {
+    constexpr bool WIDE = !BF16;
+    constexpr int WAVES = WN * WM, BN = 16 * NT * WN, BM = 16 * MT * WM, ROWS = BN + BM, PIECES = ROWS / 8 / WAVES;
+    __shared__ u32x4 lds[2 * ROWS * 8];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int tn, tm;
+    if (!tile_of(tiles_n, tiles_m, tn, tm)) return;
+    const int n0 = tn * BN, m0 = tm * BM;
+    const int wn = (wave % WN) * 16 * NT, wm = (wave / WN) * 16 * MT;
+    const int r16 = lane & 15, g = lane >> 4;
+    const uint8_t* row[PIECES];
+    u32x4 held[PIECES];
+    auto piece_row = [&](int i) { return (wave + i * WAVES) * 8 + (lane >> 3); };
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int r = piece_row(i);
+        row[i] = r < BN ? P.W + (long)(n0 + r < P.N ? n0 + r : P.N - 1) * P.ldw : P.X + (long)(m0 + r - BN < P.M ? m0 + r - BN : P.M - 1) * P.ldx;
+    }
+    auto fetch = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int r = piece_row(i);
+            const int c = r < BN ? (lane & 7) ^ w_place<NT>(r) : (lane & 7) ^ ((r - BN) & 7);
+            held[i] = row_chunk(row[i], b * 128 + c * 16, P.K);
+        }
+    };
+    auto store_held = [&](int stage) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) lds[(stage * ROWS + piece_row(i)) * 8 + (lane & 7)] = held[i];
+    };
+    const float* xs[MT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        const int m = m0 + wm + 16 * j + r16;
+        xs[j] = P.XS + (long)(m < P.M ? m : P.M - 1) * P.xs_row;
+    }
+    const int nb = (n0 + wn) >> 7, nb_last = (P.N - 1) >> 7;
+    const float* const ws = P.WS + (long)(nb < nb_last ? nb : nb_last) * P.KB;
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    fetch(0);
+    store_held(0);
+    for (int b = 0; b < P.KB; ++b) {
+        const int stage = b & 1;
+        float s[MT];
+#pragma unroll
+        for (int j = 0; j < MT; ++j) s[j] = ws[b] * xs[j][(long)b * P.xs_blk];
+        __syncthreads();                               // the block is there; the other stage is no longer read
+        if (b + 1 < P.KB) fetch(b + 1);
+        const u32x4* const base = lds + stage * ROWS * 8;
+        Frag<WIDE> fx[MT];
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            const int r = BN + wm + 16 * j + r16, f = r16 & 7;
+            fx[j] = make_frag<WIDE>(base[r * 8 + (g ^ f)], base[r * 8 + ((g + 4) ^ f)]);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int r = wn + 4 * NT * (r16 >> 2) + 4 * t + (r16 & 3), f = w_place<NT>(r);
+            const Frag<WIDE> fw = make_frag<WIDE>(base[r * 8 + (g ^ f)], base[r * 8 + ((g + 4) ^ f)]);
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                const f32x4 p = block_product<WIDE>(fw, fx[j]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[t][j][k] = fmaf(p[k], s[j], acc[t][j][k]);
+            }
+        }
+        if (b + 1 < P.KB) store_held(stage ^ 1);
+    }
+    store_tile<NT, MT, BF16>(P, acc, n0 + wn, m0 + wm, r16, g);
+}
+
+// ---- few rows: 16 NT outputs n x 16 MT rows m per workgroup; its WV waves share the blocks of K ------------------------------
+// Bound by reading the weights: every wave reads the 16 NT weight rows of its blocks straight into registers (16 bytes per lane
+// and load, any alignment), U blocks at a time so that their loads are in flight together; the partial sums of the waves are
+// joined in wave order through LDS.
+template <int MT, int NT, int U, int WV, bool BF16>
+__global__ __launch_bounds__(64 * WV) void fp8_mix_few_kernel(const MixArgs P) {
+    constexpr bool WIDE = !BF16;
+    __shared__ float part[WV][NT * MT * 4][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
+    const int r16 = lane & 15, g = lane >> 4;
+    const uint8_t* w[NT];
     const uint8_t* x[MT];
     const float* xs[MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) w[t] = P.W + (long)(n0 + 16 * t + r16 < P.N ? n0 + 16 * t + r16 : P.N - 1) * P.ldw;
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
         const int m = m0 + 16 * j + r16 < P.M ? m0 + 16 * j + r16 : P.M - 1;
         x[j] = P.X + (long)m * P.ldx;
         xs[j] = P.XS + (long)m * P.xs_row;
     }
-    const float* const ws = P.WS + (long)(n0 >> 7) * P.KB;
-    f32x4 acc[MT];
+    const float* const ws = P.WS + (long)(n0 >> 7) * P.KB;      // (16 NT divides 128: the outputs share a row of scales)
+    f32x4 acc[NT][MT];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto add = [&](const u32x4 (&wc)[2], const u32x4 (&xc)[MT][2], float sw, const float (&sx)[MT]) {
-        const Frag<WIDE> fw = make_frag<WIDE>(wc[0], wc[1]);
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto add = [&](const u32x4 (&wc)[NT][2], const u32x4 (&xc)[MT][2], float sw, const float (&sx)[MT]) {
+        Frag<WIDE> fw[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) fw[t] = make_frag<WIDE>(wc[t][0], wc[t][1]);
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-            const f32x4 p = block_product<WIDE>(fw, make_frag<WIDE>(xc[j][0], xc[j][1]));
+            const Frag<WIDE> fx = make_frag<WIDE>(xc[j][0], xc[j][1]);
             const float s = sw * sx[j];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) acc[j][q] = fmaf(p[q], s, acc[j][q]);
+            for (int t = 0; t < NT; ++t) {
+                const f32x4 p = block_product<WIDE>(fw[t], fx);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[t][j][q] = fmaf(p[q], s, acc[t][j][q]);
+            }
         }
     };
     const int whole = P.K >> 7;
-    for (int b0 = wave; b0 < whole; b0 += FEW_WAVES * U) {
-        u32x4 wc[U][2], xc[U][MT][2];
+    for (int b0 = wave; b0 < whole; b0 += WV * U) {
+        u32x4 wc[U][NT][2], xc[U][MT][2];
         float sw[U], sx[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int b = b0 + u * FEW_WAVES;
+            const int b = b0 + u * WV;
             if (b < whole) {                           // (uniform)
                 const long k = (long)b * 128 + g * 16;
-                wc[u][0] = chunk(w + k);
-                wc[u][1] = chunk(w + k + 64);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) { wc[u][t][0] = chunk(w[t] + k); wc[u][t][1] = chunk(w[t] + k + 64); }
                 sw[u] = ws[b];
 #pragma unroll
                 for (int j = 0; j < MT; ++j) {
@@ -340,12 +474,14 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void fp8_mix_few_kernel(const MixAr
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (b0 + u * FEW_WAVES < whole) add(wc[u], xc[u], sw[u], sx[u]);
+            if (b0 + u * WV < whole) add(wc[u], xc[u], sw[u], sx[u]);
     }
-    if (whole < P.KB && wave == whole % FEW_WAVES) {   // the short last block, by the wave whose turn it is
+    if (whole < P.KB && wave == whole % WV) {          // the short last block, by the wave whose turn it is
         const int k = whole * 128 + g * 16;
-        u32x4 wc[2] = {row_chunk(w, k, P.K), row_chunk(w, k + 64, P.K)}, xc[MT][2];
+        u32x4 wc[NT][2], xc[MT][2];
         float sx[MT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) { wc[t][0] = row_chunk(w[t], k, P.K); wc[t][1] = row_chunk(w[t], k + 64, P.K); }
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
             xc[j][0] = row_chunk(x[j], k, P.K);
@@ -355,17 +491,19 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void fp8_mix_few_kernel(const MixAr
         add(wc, xc, ws[whole], sx);
     }
 #pragma unroll
-    for (int j = 0; j < MT; ++j)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) part[wave][4 * j + q][lane] = acc[j][q];
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) part[wave][(t * MT + j) * 4 + q][lane] = acc[t][j][q];
     __syncthreads();
-    // output (n, m) of the tile: lane 16 (n / 4) + m % 16 of register 4 (m / 16) + n % 4
-    for (int e = threadIdx.x; e < 256 * MT; e += 64 * FEW_WAVES) {
-        const int n = e & 15, m = e >> 4;
-        const int reg = 4 * (m >> 4) + (n & 3), l = 16 * (n >> 2) + (m & 15);
+    // output (n, m) of the tile: lane 16 (n % 16 / 4) + m % 16 of register 4 (MT (n / 16) + m / 16) + n % 4
+    for (int e = threadIdx.x; e < 256 * NT * MT; e += 64 * WV) {
+        const int n = e % (16 * NT), m = e / (16 * NT);
+        const int reg = 4 * (MT * (n >> 4) + (m >> 4)) + (n & 3), l = 16 * ((n & 15) >> 2) + (m & 15);
         float v = 0.f;
 #pragma unroll
-        for (int q = 0; q < FEW_WAVES; ++q) v += part[q][reg][l];
+        for (int q = 0; q < WV; ++q) v += part[q][reg][l];
         if (m0 + m < P.M && n0 + n < P.N) {
             if (P.bias != nullptr) v += load_out<BF16>(P.bias, n0 + n);
             store_out<BF16>(P.Y, (long)(m0 + m) * P.N + n0 + n, v);
@@ -373,12 +511,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void fp8_mix_few_kernel(const MixAr
     }
 }
 
-template <int NT, int MT, int WN, int WM, bool BF16, bool DMA>
+template <int NT, int MT, int WN, int WM, bool BF16>
 static int launch_tile(const MixArgs& a, hipStream_t s) {
     constexpr int BN = 16 * NT * WN, BM = 16 * MT * WM;
     const int tn = (a.N + BN - 1) / BN, tm = (a.M + BM - 1) / BM;
-    const int lds = 2 * (BN + BM) * 128;
-    auto* kernel = fp8_mix_tile_kernel<NT, MT, WN, WM, BF16, DMA>;
+    constexpr int lds = 2 * ((BN + BM) * 128 + WN * WM * 256);
+    static_assert(lds <= 160 * 1024, "");
+    auto* kernel = fp8_mix_tile_kernel<NT, MT, WN, WM, BF16>;
     if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
         return DSW_ERR_LAUNCH;
     const long per = ((long)tn * tm + 7) / 8;
@@ -386,25 +525,52 @@ static int launch_tile(const MixArgs& a, hipStream_t s) {
     return dsw_check_launch();
 }
 template <bool BF16>
+static int launch_any(const MixArgs& a, hipStream_t s) {
+    const int tn = (a.N + 127) / 128, tm = (a.M + 127) / 128;
+    const long per = ((long)tn * tm + 7) / 8;
+    DSW_LAUNCH((fp8_mix_any_kernel<4, 4, 2, 2, BF16>), dim3((unsigned)(per * 8)), dim3(256), 0, s, a, tn, tm);
+    return dsw_check_launch();
+}
+template <bool BF16>
 static int launch_few(const MixArgs& a, hipStream_t s) {
-    const unsigned gn = (unsigned)((a.N + 15) / 16);
-#define FEW(MT_, U_) DSW_LAUNCH((fp8_mix_few_kernel<MT_, U_, BF16>), dim3(gn, (unsigned)((a.M + 16 * MT_ - 1) / (16 * MT_))), dim3(64 * FEW_WAVES), 0, s, a)
-    if (a.M <= 16) FEW(1, 4);
-    else if (a.M <= 32) FEW(2, 2);
-    else if (a.M <= 48) FEW(3, 2);
-    else FEW(4, 2);
+#define FEW(...) FEW_(__VA_ARGS__)
+#define FEW_(MT_, NT_, U_, WV_) \
+    DSW_LAUNCH((fp8_mix_few_kernel<MT_, NT_, U_, WV_, BF16>), dim3((unsigned)((a.N + 16 * NT_ - 1) / (16 * NT_)), (unsigned)((a.M + 16 * MT_ - 1) / (16 * MT_))), \
+               dim3(64 * WV_), 0, s, a)
+#ifndef FEW1
+#define FEW1 1, 1, 4, 8
+#define FEW2 2, 1, 2, 8
+#define FEW3 3, 1, 2, 8
+#define FEW4 4, 1, 2, 8
+#endif
+    if (a.M <= 16) FEW(FEW1);
+    else if (a.M <= 32) FEW(FEW2);
+    else if (a.M <= 48) FEW(FEW3);
+    else FEW(FEW4);
 #undef FEW
+#undef FEW_
     return dsw_check_launch();
 }
 template <bool BF16>
 static int launch_mix(const MixArgs& a, hipStream_t s) {
     const bool dma = a.K % 16 == 0 && a.ldx % 16 == 0 && a.ldw % 16 == 0 && dsw_aligned16(a.X) && dsw_aligned16(a.W);
     if (a.M <= 64 || (long)((a.M + 127) / 128) * ((a.N + 127) / 128) < 64) return launch_few<BF16>(a, s);
-    if (!dma) return launch_tile<4, 4, 2, 2, BF16, false>(a, s);
+    if (!dma) return launch_any<BF16>(a, s);
+#ifndef BIG_TILE
+#define BIG_TILE 8, 4, 2, 4
+#define MID_TILE 4, 4, 2, 2
+#define BIG_N 256
+#define BIG_M 256
+#endif
+#ifndef WIDE_TILE
+#define WIDE_TILE 4, 2, 2, 4
+#endif
     if constexpr (BF16) {
-        if ((long)((a.M + 255) / 256) * ((a.N + 255) / 256) >= 256) return launch_tile<8, 4, 2, 4, BF16, true>(a, s);
+        if ((long)((a.M + BIG_M - 1) / BIG_M) * ((a.N + BIG_N - 1) / BIG_N) >= 256) return launch_tile<BIG_TILE, BF16>(a, s);
+        return launch_tile<MID_TILE, BF16>(a, s);
+    } else {
+        return launch_tile<WIDE_TILE, BF16>(a, s);
     }
-    return launch_tile<4, 4, 2, 2, BF16, true>(a, s);
 }
 
 }  // namespace
