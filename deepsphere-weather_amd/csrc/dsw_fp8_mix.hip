@@ -134,9 +134,13 @@ static __device__ __forceinline__ bool tile_of(int tiles_n, int tiles_m, int& tn
     return true;
 }
 
-// a wave's results: lane (r16, g) holds outputs n0 + 4 NT g .. + 4 NT - 1 of the rows m0 + 16 j + r16
+// A wave's results: lane (r16, g) holds outputs n0 + 4 NT g .. + 4 NT - 1 of the rows m0 + 16 j + r16.  Written as they lie, a store
+// would be 64 pieces of 16 bytes in as many lines (measured: 134 MB at 2.4 TB/s); they are turned in the wave's own part of LDS
+// (16-byte chunks, chunk c of row m at place c ^ m) and leave as whole runs of a row.
 template <int NT, int MT, bool BF16>
-static __device__ __forceinline__ void store_tile(const MixArgs& P, const f32x4 (&acc)[NT][MT], int n0, int m0, int r16, int g) {
+static __device__ __forceinline__ void store_tile(const MixArgs& P, const f32x4 (&acc)[NT][MT], u32x4* own, int n0, int m0, int lane) {
+    constexpr int PER = BF16 ? 8 : 4, CH = 16 * NT / PER;        // outputs of a chunk, chunks of a row
+    const int r16 = lane & 15, g = lane >> 4;
     const int n = n0 + 4 * NT * g;
     float add[4 * NT];
 #pragma unroll
@@ -145,39 +149,38 @@ static __device__ __forceinline__ void store_tile(const MixArgs& P, const f32x4 
 #pragma unroll
         for (int k = 0; k < 4 * NT; ++k) add[k] = n + k < P.N ? load_out<BF16>(P.bias, n + k) : 0.f;
     }
-    const bool vec = n + 4 * NT <= P.N && P.N % 8 == 0 && ((uintptr_t)P.Y & 15) == 0;
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
-        const int m = m0 + 16 * j + r16;
-        if (m >= P.M) continue;
-        const long at = (long)m * P.N + n;
-        if (vec) {
-            if constexpr (BF16) {
+        const int m = 16 * j + r16;
 #pragma unroll
-                for (int t = 0; t < NT; t += 2) {
-                    u32x4 v;
+        for (int c = 0; c < CH / 4; ++c) {
+            u32x4 v;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int e = t * 4 + 2 * q;
-                        v[q] = f32_to_bf16(acc[e / 4][j][e % 4] + add[e]) | (uint32_t)f32_to_bf16(acc[e / 4][j][e % 4 + 1] + add[e + 1]) << 16;
-                    }
-                    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(P.Y) + at + 4 * t) = v;
-                }
-            } else {
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    f32x4 v = acc[t][j];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) v[q] += add[4 * t + q];
-                    *reinterpret_cast<f32x4*>(static_cast<float*>(P.Y) + at + 4 * t) = v;
+            for (int q = 0; q < 4; ++q) {
+                if constexpr (BF16) {
+                    const int e = c * 8 + 2 * q;
+                    v[q] = f32_to_bf16(acc[e / 4][j][e % 4] + add[e]) | (uint32_t)f32_to_bf16(acc[e / 4][j][e % 4 + 1] + add[e + 1]) << 16;
+                } else {
+                    v[q] = __float_as_uint(acc[c][j][q] + add[4 * c + q]);
                 }
             }
+            own[m * CH + ((g * (CH / 4) + c) ^ (m & (CH - 1)))] = v;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16 * MT * CH / 64; ++i) {
+        const int e = i * 64 + lane, row = e / CH, c = e % CH;
+        const u32x4 v = own[row * CH + (c ^ (row & (CH - 1)))];
+        const int m = m0 + row, k = n0 + c * PER;
+        if (m >= P.M || k >= P.N) continue;
+        const long at = (long)m * P.N + k;
+        if (k + PER <= P.N) {
+            reinterpret_cast<Any16*>(static_cast<char*>(P.Y) + at * (16 / PER))->v = v;
         } else {
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (n + 4 * t + q < P.N) store_out<BF16>(P.Y, at + 4 * t + q, acc[t][j][q] + add[4 * t + q]);
+            for (int q = 0; q < P.N - k; ++q) {
+                if constexpr (BF16) static_cast<uint16_t*>(P.Y)[at + q] = (uint16_t)(v[q >> 1] >> (16 * (q & 1)));
+                else static_cast<uint32_t*>(P.Y)[at + q] = v[q];
+            }
         }
     }
 }
@@ -328,7 +331,10 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
             }
         }
     }
-    store_tile<NT, MT, BF16>(P, acc, n0 + wn, m0 + wm, r16, g);
+    __syncthreads();
+    constexpr int OWN = 16 * NT * 16 * MT / (BF16 ? 8 : 4);      // 16-byte chunks of a wave's results
+    static_assert(WAVES * OWN <= 2 * STAGE, "the results fit the stages");
+    store_tile<NT, MT, BF16>(P, acc, lds + wave * OWN, n0 + wn, m0 + wm, lane);
 }
 
 // any alignment and strides: the same tiles, two stages, filled through registers
@@ -405,7 +411,10 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_any_kernel(const MixArgs
         }
         if (b + 1 < P.KB) store_held(stage ^ 1);
     }
-    store_tile<NT, MT, BF16>(P, acc, n0 + wn, m0 + wm, r16, g);
+    __syncthreads();
+    constexpr int OWN = 16 * NT * 16 * MT / (BF16 ? 8 : 4);
+    static_assert(WAVES * OWN <= 2 * ROWS * 8, "the results fit the stages");
+    store_tile<NT, MT, BF16>(P, acc, lds + wave * OWN, n0 + wn, m0 + wm, lane);
 }
 
 // ---- few rows: 16 NT outputs n x 16 MT rows m per workgroup; its WV waves share the blocks of K ------------------------------
