@@ -137,7 +137,8 @@ static __device__ __forceinline__ bool tile_of(int tiles_n, int tiles_m, int& tn
 // A wave's results: lane (r16, g) holds outputs n0 + 4 NT g .. + 4 NT - 1 of the rows m0 + 16 j + r16.  Written as they lie, a store
 // would be 64 pieces of 16 bytes in as many lines (measured: 134 MB at 2.4 TB/s); they are turned in the wave's own part of LDS
 // (16-byte chunks, chunk c of row m at place c ^ m) and leave as whole runs of a row.
-template <int NT, int MT, bool BF16>
+// STREAM: the output is far larger than the caches and leaves past them.
+template <int NT, int MT, bool BF16, bool STREAM>
 static __device__ __forceinline__ void store_tile(const MixArgs& P, const f32x4 (&acc)[NT][MT], u32x4* own, int n0, int m0, int lane) {
     constexpr int PER = BF16 ? 8 : 4, CH = 16 * NT / PER;        // outputs of a chunk, chunks of a row
     const int r16 = lane & 15, g = lane >> 4;
@@ -167,6 +168,7 @@ static __device__ __forceinline__ void store_tile(const MixArgs& P, const f32x4 
             own[m * CH + ((g * (CH / 4) + c) ^ (m & (CH - 1)))] = v;
         }
     }
+    const bool whole_chunks = P.N % PER == 0 && ((uintptr_t)P.Y & 15) == 0;
 #pragma unroll
     for (int i = 0; i < 16 * MT * CH / 64; ++i) {
         const int e = i * 64 + lane, row = e / CH, c = e % CH;
@@ -175,7 +177,9 @@ static __device__ __forceinline__ void store_tile(const MixArgs& P, const f32x4 
         if (m >= P.M || k >= P.N) continue;
         const long at = (long)m * P.N + k;
         if (k + PER <= P.N) {
-            reinterpret_cast<Any16*>(static_cast<char*>(P.Y) + at * (16 / PER))->v = v;
+            char* const y = static_cast<char*>(P.Y) + at * (16 / PER);
+            if (STREAM && whole_chunks) __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(y));
+            else reinterpret_cast<Any16*>(y)->v = v;
         } else {
             for (int q = 0; q < P.N - k; ++q) {
                 if constexpr (BF16) static_cast<uint16_t*>(P.Y)[at + q] = (uint16_t)(v[q >> 1] >> (16 * (q & 1)));
@@ -186,9 +190,9 @@ static __device__ __forceinline__ void store_tile(const MixArgs& P, const f32x4 
 }
 
 // 16-byte aligned rows of whole 16-byte chunks: two stages in LDS, filled without registers.  One meeting per block, before its
-// last step t: by then every wave has read its last weights of the block, so its stage takes the loads of the block after next,
-// and the next block has landed (its loads had a whole block's time), so its first fragments are read while the last step's
-// products are computed.  The matrix cores thus wait neither for the barrier nor for the fragments behind it.
+// last step t: by then every wave has read its last weights of the block, so its stage takes the loads of the block after next
+// (issued at once: they have a whole block's time), and the next block has landed, so its first fragments are read while the
+// last step's products are computed.  The matrix cores thus wait neither for the barrier nor for the fragments behind it.
 // The products of one step are scaled and added while the next step's are computed: a 16x16x128 product takes 32 clocks, of which
 // the vector unit is free for 16, its four additions (measured: 4 additions a product cost 12 %, each further instruction 4
 // clocks) - so the loop's addresses are scalars and immediates.
@@ -199,7 +203,8 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
     constexpr int STAGE = ROWS * 8 + WAVES * 16;       // 16-byte units: the rows, then 64 row scales of each wave
     static_assert(ROWS % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "a wave's pieces lie in one operand each");
     static_assert(128 % (16 * NT) == 0, "a wave's outputs share a row of weight scales");
-    static_assert(MT <= 4 && NT >= 2 && NT % 2 == 0 && PIECES < (NT - 1) * MT, "every load is issued before the last step");
+    constexpr int GO = (PIECES + MT) / MT;             // loads issued with each of the last step's products
+    static_assert(MT <= 4 && NT >= 2 && NT % 2 == 0, "");
     extern __shared__ u32x4 lds[];                     // [2][STAGE]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int tn, tm;
@@ -252,7 +257,11 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
         for (int i = 0; i < PIECES; ++i) fetch_piece(i, off[i], 0);
         fetch_scales(0);
         advance(whole > 1);
-        wait_loads();
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) fetch_piece(i, off[i], 1);
+        fetch_scales(1);
+        advance(whole > 2);
+        asm volatile("s_waitcnt vmcnt(%0)" :: "n"(PIECES + 1) : "memory");     // block 0 is there, block 1 on its way
         __syncthreads();
         Frag<WIDE> fx[MT], fw = make_frag<WIDE>(lds[w_lo], lds[w_hi]);
         float s[MT], s_old[MT];
@@ -263,7 +272,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
             s_old[j] = 0.f;
         }
         // No branch in the loop (the additions have to stay between the products): behind the last block it fetches that block
-        // again, into the stage that nobody reads any more.
+        // again, into stages that nobody reads any more.
         int stage = 0;
         for (int b = 0; b < whole; ++b) {
             const u32x4* const here = lds + stage * STAGE;
@@ -287,9 +296,14 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
                     const f32x4 q = p[j];
                     const float sq = t == 0 ? s_old[j] : s[j];
                     p[j] = block_product<WIDE>(fw, fx[j]);
-                    if (t * MT + j < PIECES) fetch_piece(t * MT + j, off[t * MT + j], stage ^ 1);
-                    if (t * MT + j == PIECES) fetch_scales(stage ^ 1);
-                    if (t + 1 == NT) fx[j] = make_frag<WIDE>(there[x_lo + 128 * j], there[x_hi + 128 * j]);
+                    if (t + 1 == NT) {
+                        fx[j] = make_frag<WIDE>(there[x_lo + 128 * j], there[x_hi + 128 * j]);
+#pragma unroll
+                        for (int i = j * GO; i < (j + 1) * GO; ++i) {          // block b + 2
+                            if (i < PIECES) fetch_piece(i, off[i], stage);
+                            else if (i == PIECES) fetch_scales(stage);
+                        }
+                    }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) acc[(t + NT - 1) % NT][j][k] = fmaf(q[k], sq, acc[(t + NT - 1) % NT][j][k]);
                     __builtin_amdgcn_sched_barrier(0);
@@ -298,9 +312,10 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
             }
 #pragma unroll
             for (int j = 0; j < MT; ++j) { s_old[j] = s[j]; s[j] = s_next[j]; }
-            advance(b + 2 < whole);
+            advance(b + 3 < whole);
             stage ^= 1;
         }
+        wait_loads();
 #pragma unroll
         for (int j = 0; j < MT; ++j)
 #pragma unroll
@@ -334,87 +349,17 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
     __syncthreads();
     constexpr int OWN = 16 * NT * 16 * MT / (BF16 ? 8 : 4);      // 16-byte chunks of a wave's results
     static_assert(WAVES * OWN <= 2 * STAGE, "the results fit the stages");
-    store_tile<NT, MT, BF16>(P, acc, lds + wave * OWN, n0 + wn, m0 + wm, lane);
+    store_tile<NT, MT, BF16, WAVES * NT * MT >= 256>(P, acc, lds + wave * OWN, n0 + wn, m0 + wm, lane);
 }
 
-// any alignment and strides: the same tiles, two stages, filled through registers
-template <int NT, int MT, int WN, int WM, bool BF16>
-__global__ __launch_bounds__(64 * WN * WM) void fp8_mix_any_kernel(const MixArgs P, const int tiles_n, const int tiles_m) {
-    constexpr bool WIDE = !BF16;
-    constexpr int WAVES = WN * WM, BN = 16 * NT * WN, BM = 16 * MT * WM, ROWS = BN + BM, PIECES = ROWS / 8 / WAVES;
-    __shared__ u32x4 lds[2 * ROWS * 8];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int tn, tm;
-    if (!tile_of(tiles_n, tiles_m, tn, tm)) return;
-    const int n0 = tn * BN, m0 = tm * BM;
-    const int wn = (wave % WN) * 16 * NT, wm = (wave / WN) * 16 * MT;
-    const int r16 = lane & 15, g = lane >> 4;
-    const uint8_t* row[PIECES];
-    u32x4 held[PIECES];
-    auto piece_row = [&](int i) { return (wave + i * WAVES) * 8 + (lane >> 3); };
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-        const int r = piece_row(i);
-        row[i] = r < BN ? P.W + (long)(n0 + r < P.N ? n0 + r : P.N - 1) * P.ldw : P.X + (long)(m0 + r - BN < P.M ? m0 + r - BN : P.M - 1) * P.ldx;
+// rows of any alignment and length -> rows of whole 16-byte chunks, zero behind the row; then the kernels above take them
+__global__ __launch_bounds__(256) void fp8_align_rows_kernel(const uint8_t* X, long ld, int K, uint8_t* out, long rows, int chunks) {
+    const long total = rows * chunks;
+    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long)gridDim.x * 256) {
+        const long r = e / chunks;
+        const int c = (int)(e - r * chunks);
+        reinterpret_cast<u32x4*>(out)[e] = row_chunk(X + r * ld, c * 16, K);
     }
-    auto fetch = [&](int b) {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int r = piece_row(i);
-            const int c = r < BN ? (lane & 7) ^ w_place<NT>(r) : (lane & 7) ^ ((r - BN) & 7);
-            held[i] = row_chunk(row[i], b * 128 + c * 16, P.K);
-        }
-    };
-    auto store_held = [&](int stage) {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) lds[(stage * ROWS + piece_row(i)) * 8 + (lane & 7)] = held[i];
-    };
-    const float* xs[MT];
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-        const int m = m0 + wm + 16 * j + r16;
-        xs[j] = P.XS + (long)(m < P.M ? m : P.M - 1) * P.xs_row;
-    }
-    const int nb = (n0 + wn) >> 7, nb_last = (P.N - 1) >> 7;
-    const float* const ws = P.WS + (long)(nb < nb_last ? nb : nb_last) * P.KB;
-    f32x4 acc[NT][MT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    fetch(0);
-    store_held(0);
-    for (int b = 0; b < P.KB; ++b) {
-        const int stage = b & 1;
-        float s[MT];
-#pragma unroll
-        for (int j = 0; j < MT; ++j) s[j] = ws[b] * xs[j][(long)b * P.xs_blk];
-        __syncthreads();                               // the block is there; the other stage is no longer read
-        if (b + 1 < P.KB) fetch(b + 1);
-        const u32x4* const base = lds + stage * ROWS * 8;
-        Frag<WIDE> fx[MT];
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-            const int r = BN + wm + 16 * j + r16, f = r16 & 7;
-            fx[j] = make_frag<WIDE>(base[r * 8 + (g ^ f)], base[r * 8 + ((g + 4) ^ f)]);
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int r = wn + 4 * NT * (r16 >> 2) + 4 * t + (r16 & 3), f = w_place<NT>(r);
-            const Frag<WIDE> fw = make_frag<WIDE>(base[r * 8 + (g ^ f)], base[r * 8 + ((g + 4) ^ f)]);
-#pragma unroll
-            for (int j = 0; j < MT; ++j) {
-                const f32x4 p = block_product<WIDE>(fw, fx[j]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[t][j][k] = fmaf(p[k], s[j], acc[t][j][k]);
-            }
-        }
-        if (b + 1 < P.KB) store_held(stage ^ 1);
-    }
-    __syncthreads();
-    constexpr int OWN = 16 * NT * 16 * MT / (BF16 ? 8 : 4);
-    static_assert(WAVES * OWN <= 2 * ROWS * 8, "the results fit the stages");
-    store_tile<NT, MT, BF16>(P, acc, lds + wave * OWN, n0 + wn, m0 + wm, lane);
 }
 
 // ---- few rows: 16 NT outputs n x 16 MT rows m per workgroup; its WV waves share the blocks of K ------------------------------
@@ -520,6 +465,103 @@ __global__ __launch_bounds__(64 * WV) void fp8_mix_few_kernel(const MixArgs P) {
     }
 }
 
+// The same split for 16-byte aligned rows of whole 16-byte chunks and more than 16 rows m: a lane's share of a fragment lies in 16
+// rows' lines, so reading it straight into registers asks for 64 lines a load (measured: 15 bytes a clock and CU, and the rows m
+// are read again by every workgroup); here each wave has its block's rows brought into its own part of LDS, 8 whole lines a
+// load, reads its fragments there and sends for its next block before it multiplies.  No wave waits for another until the sums
+// are joined.
+template <int MT, int NT, int WV, bool BF16>
+__global__ __launch_bounds__(64 * WV) void fp8_mix_few_lds_kernel(const MixArgs P) {
+    constexpr bool WIDE = !BF16;
+    constexpr int ROWS = 16 * (NT + MT);
+    extern __shared__ u32x4 lds[];                     // [WV][ROWS][8], then [WV][NT MT 4][64] sums in the same place
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
+    const int r16 = lane & 15, g = lane >> 4;
+    const uint8_t* const wbase = P.W + (long)n0 * P.ldw;
+    const uint8_t* const xbase = P.X + (long)m0 * P.ldx;
+    uint32_t off[ROWS / 8];
+    const int c16 = ((lane & 7) ^ (lane >> 3)) * 16;   // row r of 8: chunk c at place c ^ r
+#pragma unroll
+    for (int i = 0; i < ROWS / 8; ++i) {
+        const int r = 8 * i + (lane >> 3);
+        if (i < 2 * NT) off[i] = (uint32_t)((n0 + r < P.N ? r : P.N - 1 - n0) * P.ldw) + c16;
+        else off[i] = (uint32_t)((m0 + r - 16 * NT < P.M ? r - 16 * NT : P.M - 1 - m0) * P.ldx) + c16;
+    }
+    const float* xs[MT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) xs[j] = P.XS + (long)(m0 + 16 * j + r16 < P.M ? m0 + 16 * j + r16 : P.M - 1) * P.xs_row;
+    const float* const ws = P.WS + (long)(n0 >> 7) * P.KB;
+    u32x4* const own = lds + wave * ROWS * 8;
+    const uint32_t to = lds_byte(lds) + (uint32_t)(wave * ROWS * 128);
+    const int whole = P.K >> 7, tail = P.K & 127;
+    auto fetch = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < ROWS / 8; ++i)
+            load_to_lds((i < 2 * NT ? wbase : xbase) + (long)b * 128, b < whole || c16 < tail ? off[i] : off[i] - c16, to + 1024 * i);
+    };
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (wave < P.KB) fetch(wave);
+    for (int b = wave; b < P.KB; b += WV) {
+        float s[MT];
+        const float sw = scalar_load(ws, b);
+#pragma unroll
+        for (int j = 0; j < MT; ++j) s[j] = xs[j][(long)b * P.xs_blk];
+        wait_loads();
+        if (b == whole && c16 >= tail) {               // the short last block: clear what lies behind the rows
+#pragma unroll
+            for (int i = 0; i < ROWS / 8; ++i) own[64 * i + lane] = u32x4{0u, 0u, 0u, 0u};
+        }
+        const int lo = r16 * 8 + (g ^ (r16 & 7)), hi = r16 * 8 + ((g + 4) ^ (r16 & 7));
+        u32x4 wc[NT][2], xc[MT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) { wc[t][0] = own[128 * t + lo]; wc[t][1] = own[128 * t + hi]; }
+#pragma unroll
+        for (int j = 0; j < MT; ++j) { xc[j][0] = own[128 * (NT + j) + lo]; xc[j][1] = own[128 * (NT + j) + hi]; }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the fragments are in registers: their place may be filled again
+        __builtin_amdgcn_sched_barrier(0);
+        if (b + WV < P.KB) fetch(b + WV);
+        Frag<WIDE> fw[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) fw[t] = make_frag<WIDE>(wc[t][0], wc[t][1]);
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            const Frag<WIDE> fx = make_frag<WIDE>(xc[j][0], xc[j][1]);
+            const float sj = sw * s[j];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const f32x4 p = block_product<WIDE>(fw[t], fx);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[t][j][q] = fmaf(p[q], sj, acc[t][j][q]);
+            }
+        }
+    }
+    __syncthreads();
+    float* const part = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) part[(wave * NT * MT * 4 + (t * MT + j) * 4 + q) * 64 + lane] = acc[t][j][q];
+    __syncthreads();
+    for (int e = threadIdx.x; e < 256 * NT * MT; e += 64 * WV) {
+        const int n = e % (16 * NT), m = e / (16 * NT);
+        const int reg = 4 * (MT * (n >> 4) + (m >> 4)) + (n & 3), l = 16 * ((n & 15) >> 2) + (m & 15);
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < WV; ++q) v += part[(q * NT * MT * 4 + reg) * 64 + l];
+        if (m0 + m < P.M && n0 + n < P.N) {
+            if (P.bias != nullptr) v += load_out<BF16>(P.bias, n0 + n);
+            store_out<BF16>(P.Y, (long)(m0 + m) * P.N + n0 + n, v);
+        }
+    }
+}
+
 template <int NT, int MT, int WN, int WM, bool BF16>
 static int launch_tile(const MixArgs& a, hipStream_t s) {
     constexpr int BN = 16 * NT * WN, BM = 16 * MT * WM;
@@ -533,77 +575,107 @@ static int launch_tile(const MixArgs& a, hipStream_t s) {
     DSW_LAUNCH(kernel, dim3((unsigned)(per * 8)), dim3(64 * WN * WM), lds, s, a, tn, tm);
     return dsw_check_launch();
 }
-template <bool BF16>
-static int launch_any(const MixArgs& a, hipStream_t s) {
-    const int tn = (a.N + 127) / 128, tm = (a.M + 127) / 128;
-    const long per = ((long)tn * tm + 7) / 8;
-    DSW_LAUNCH((fp8_mix_any_kernel<4, 4, 2, 2, BF16>), dim3((unsigned)(per * 8)), dim3(256), 0, s, a, tn, tm);
-    return dsw_check_launch();
-}
-template <bool BF16>
+template <int MT, int NT, int U, int WV, bool BF16>
 static int launch_few(const MixArgs& a, hipStream_t s) {
-#define FEW(...) FEW_(__VA_ARGS__)
-#define FEW_(MT_, NT_, U_, WV_) \
-    DSW_LAUNCH((fp8_mix_few_kernel<MT_, NT_, U_, WV_, BF16>), dim3((unsigned)((a.N + 16 * NT_ - 1) / (16 * NT_)), (unsigned)((a.M + 16 * MT_ - 1) / (16 * MT_))), \
-               dim3(64 * WV_), 0, s, a)
-#ifndef FEW1
-#define FEW1 1, 1, 4, 8
-#define FEW2 2, 1, 2, 8
-#define FEW3 3, 1, 2, 8
-#define FEW4 4, 1, 2, 8
-#endif
-    if (a.M <= 16) FEW(FEW1);
-    else if (a.M <= 32) FEW(FEW2);
-    else if (a.M <= 48) FEW(FEW3);
-    else FEW(FEW4);
-#undef FEW
-#undef FEW_
+    DSW_LAUNCH((fp8_mix_few_kernel<MT, NT, U, WV, BF16>), dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT))),
+               dim3(64 * WV), 0, s, a);
     return dsw_check_launch();
 }
+template <int MT, int NT, int WV, bool BF16>
+static int launch_few_lds(const MixArgs& a, hipStream_t s) {
+    constexpr int stage = WV * 16 * (NT + MT) * 128, sums = WV * NT * MT * 1024, lds = stage > sums ? stage : sums;
+    auto* kernel = fp8_mix_few_lds_kernel<MT, NT, WV, BF16>;
+    if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+        return DSW_ERR_LAUNCH;
+    DSW_LAUNCH(kernel, dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT))), dim3(64 * WV), lds, s, a);
+    return dsw_check_launch();
+}
+
+static bool rows_aligned(const MixArgs& a) {
+    return a.K % 16 == 0 && a.ldx % 16 == 0 && a.ldw % 16 == 0 && dsw_aligned16(a.X) && dsw_aligned16(a.W);
+}
+// up to here rows of any alignment go through the register kernel; with more rows m aligned copies of both operands are cheaper
+constexpr int MIX_FEW_ROWS = 64;
+static int64_t mix_ws_bytes(int64_t M, int64_t N, int64_t K, bool aligned) {
+    return aligned || M <= MIX_FEW_ROWS ? 0 : (M + N) * ((K + 15) / 16 * 16);
+}
+
+// Which kernel (time in us, bf16 output, aligned rows; "LDS" = fp8_mix_few_lds_kernel<2, 1, 8>, tiles as outputs n x rows m):
+//   rows x K x N        registers  LDS   32x128  128x128  256x256
+//   8 x 4096 x 4096         6.0    6.7    18.3     22.7
+//   64 x 8192 x 1024       21.7    8.9    32.6     41.3
+//   500 x 2048 x 512        8.1    5.1     9.8     12.2     30.1
+//   1000 x 256 x 1000      11.8    8.2     4.4      5.7     12.8
+//   1000 x 4096 x 1000     47.9   26.5    19.7     24.2     52.1
+//   24576 x 256 x 256      63.4           10.8      9.0     14.6
+//   98304 x 128 x 256     219             28.1     19.5     26.6
+//   4096 x 1024 x 4096    273             44.4     27.8     26.4
+//   4096 x 4096 x 4096    737            136       80.4     65.4
+// so: 16 rows at most - registers; as long as the LDS kernel's workgroups come to four per CU - that; the larger tiles as soon as
+// there is one for every CU (the largest from six blocks of K on: below, its fuller epilogue costs more than it saves).
+// fp32 output (bf16 matrix instructions): 128 x 128 tiles of four waves instead of eight (4096^3: 134 against 149), no larger ones.
 template <bool BF16>
 static int launch_mix(const MixArgs& a, hipStream_t s) {
-    const bool dma = a.K % 16 == 0 && a.ldx % 16 == 0 && a.ldw % 16 == 0 && dsw_aligned16(a.X) && dsw_aligned16(a.W);
-    if (a.M <= 64 || (long)((a.M + 127) / 128) * ((a.N + 127) / 128) < 64) return launch_few<BF16>(a, s);
-    if (!dma) return launch_any<BF16>(a, s);
-#ifndef BIG_TILE
-#define BIG_TILE 8, 4, 2, 4
-#define MID_TILE 4, 4, 2, 2
-#define BIG_N 256
-#define BIG_M 256
-#endif
-#ifndef WIDE_TILE
-#define WIDE_TILE 4, 2, 2, 4
-#endif
-    if constexpr (BF16) {
-        if ((long)((a.M + BIG_M - 1) / BIG_M) * ((a.N + BIG_N - 1) / BIG_N) >= 256) return launch_tile<BIG_TILE, BF16>(a, s);
-        return launch_tile<MID_TILE, BF16>(a, s);
-    } else {
-        return launch_tile<WIDE_TILE, BF16>(a, s);
+    const long cus = dsw_device_cus();
+    auto tiles = [&](long n, long m) { return (a.N + n - 1) / n * ((a.M + m - 1) / m); };
+    if (a.M <= 16) return launch_few<1, 1, 4, 8, BF16>(a, s);
+    if (!rows_aligned(a)) {                            // (at most MIX_FEW_ROWS: the caller has aligned the others)
+        if (a.M <= 32) return launch_few<2, 1, 1, 8, BF16>(a, s);
+        return launch_few<4, 1, 1, 8, BF16>(a, s);
     }
+    if (tiles(16, 32) <= 4 * cus) return launch_few_lds<2, 1, 8, BF16>(a, s);
+    if constexpr (BF16) {
+        if (a.KB >= 6 && tiles(256, 256) >= cus) return launch_tile<8, 4, 2, 4, BF16>(a, s);
+        if (a.N > 64 && tiles(128, 128) >= cus) return launch_tile<4, 2, 2, 4, BF16>(a, s);
+    } else {
+        if (a.N > 64 && tiles(128, 128) >= cus) return launch_tile<4, 4, 2, 2, BF16>(a, s);
+    }
+    return launch_tile<2, 2, 1, 4, BF16>(a, s);
+}
+
+static int align_rows(const uint8_t* X, long ld, int K, uint8_t* out, long rows, hipStream_t s) {
+    const int chunks = (K + 15) / 16;
+    const long blocks = (rows * chunks + 255) / 256;
+    DSW_LAUNCH(fp8_align_rows_kernel, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, X, ld, K, out, rows, chunks);
+    return dsw_check_launch();
 }
 
 }  // namespace
 
 extern "C" {
 
-int64_t dsw_fp8_mix_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    if (M < 0 || N < 1 || K < 1 || M > 0x7fffffff - 256 || N > (1 << 22) || K > MIX_LD_MAX) return DSW_ERR_BAD_ARG;
-    return 0;
+static bool mix_sizes_ok(int64_t M, int64_t N, int64_t K) {
+    return M >= 0 && N >= 1 && K >= 1 && M <= 0x7fffffff - 256 && N <= (1 << 22) && K <= MIX_LD_MAX - 15;
+}
+
+int64_t dsw_fp8_mix_workspace_bytes(int64_t M, int64_t N, int64_t K, int aligned) {
+    if (!mix_sizes_ok(M, N, K)) return DSW_ERR_BAD_ARG;
+    return mix_ws_bytes(M, N, K, aligned != 0);
 }
 
 int dsw_fp8_mix(const void* X, int64_t ldx, const float* XS, int64_t xs_row, int64_t xs_blk, const void* W, int64_t ldw,
                 const float* WS, const void* bias, void* Y, int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
                 int64_t workspace_bytes, dsw_stream_t stream) {
     if (dtype != DSW_F32 && dtype != DSW_BF16) return DSW_ERR_BAD_DTYPE;
-    const int64_t need = dsw_fp8_mix_workspace_bytes(M, N, K);
-    if (need < 0 || ldx < K || ldw < K || ldx > MIX_LD_MAX || ldw > MIX_LD_MAX || xs_row < 0 || xs_blk < 0) return DSW_ERR_BAD_ARG;
+    if (!mix_sizes_ok(M, N, K) || ldx < K || ldw < K || ldx > MIX_LD_MAX || ldw > MIX_LD_MAX || xs_row < 0 || xs_blk < 0) return DSW_ERR_BAD_ARG;
     if (M == 0) return DSW_OK;
     if (!X || !XS || !W || !WS || !Y) return DSW_ERR_BAD_ARG;
-    if (need > 0 && (!workspace || workspace_bytes < need)) return DSW_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
+    MixArgs a{(const uint8_t*)X, XS, (const uint8_t*)W, WS, bias, Y, (long)ldx, (long)ldw, (long)xs_row, (long)xs_blk,
+              (int)M, (int)N, (int)K, (int)((K + 127) / 128)};
+    const bool aligned = rows_aligned(a);
+    const int64_t need = mix_ws_bytes(M, N, K, aligned);
+    if (need > 0 && (!workspace || workspace_bytes < need || !dsw_aligned16(workspace))) return DSW_ERR_WORKSPACE;
     DswTraceScope trace_(s, DSW_ROLE_FP8_MIX, M, K, N);
-    const MixArgs a{(const uint8_t*)X, XS, (const uint8_t*)W, WS, bias, Y, (long)ldx, (long)ldw, (long)xs_row, (long)xs_blk,
-                    (int)M, (int)N, (int)K, (int)((K + 127) / 128)};
+    if (need > 0) {
+        const long ld = (long)((K + 15) / 16 * 16);
+        uint8_t* const x = static_cast<uint8_t*>(workspace);
+        uint8_t* const w = x + M * ld;
+        int rc = align_rows(a.X, a.ldx, a.K, x, (long)M, s);
+        if (rc == DSW_OK) rc = align_rows(a.W, a.ldw, a.K, w, (long)N, s);
+        if (rc != DSW_OK) return rc;
+        a.X = x; a.W = w; a.ldx = a.ldw = ld; a.K = (int)ld;       // (zeros behind the rows; the same number of scale blocks)
+    }
     return dtype == DSW_BF16 ? launch_mix<true>(a, s) : launch_mix<false>(a, s);
 }
 

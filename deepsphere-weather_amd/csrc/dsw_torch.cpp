@@ -320,10 +320,13 @@ Tensor dense_mix_fp8(const Tensor& xq, const Tensor& xs, const Tensor& wq, const
     std::vector<int64_t> sizes(xq.sizes().begin(), xq.sizes().end());
     sizes.back() = n;
     const Tensor y = at::empty(sizes, xq.options().dtype(dtype));
-    const int64_t bytes = lib.fp8_mix_workspace_bytes(x.rows, n, k);
+    const int64_t w_step = std::max(w.stride(0), k);
+    const auto low = [](const void* p) { return (int64_t)(reinterpret_cast<uintptr_t>(p) & 15); };
+    const bool aligned = (low(x.t.data_ptr()) | low(w.data_ptr()) | ((x.step | w_step | k) & 15)) == 0;
+    const int64_t bytes = lib.fp8_mix_workspace_bytes(x.rows, n, k, aligned);
     check(bytes, "dsw_fp8_mix_workspace_bytes");
     const Tensor work = bytes ? at::empty({bytes}, xq.options().dtype(at::kByte)) : Tensor();
-    check(lib.fp8_mix(x.t.data_ptr(), x.step, s.t.data_ptr<float>(), s.step, s.t.stride(-1), w.data_ptr(), std::max(w.stride(0), k), wsc.data_ptr<float>(),
+    check(lib.fp8_mix(x.t.data_ptr(), x.step, s.t.data_ptr<float>(), s.step, s.t.stride(-1), w.data_ptr(), w_step, wsc.data_ptr<float>(),
                       b.defined() ? b.data_ptr() : nullptr, y.data_ptr(), x.rows, n, k, code, bytes ? work.data_ptr() : nullptr, bytes, stream_of(xq)),
           "dsw_fp8_mix");
     return y;

@@ -20,13 +20,23 @@ def hipcc_path():
     return "hipcc"
 
 
+HEADER = os.path.join(os.path.dirname(os.path.dirname(HERE)), "include", "dsw_hip.h")
+
+
+def _stale(out, deps):
+    return not os.path.exists(out) or any(os.path.getmtime(d) > os.path.getmtime(out) for d in deps if os.path.exists(d))
+
+
+def library_stale():
+    return _stale(OUT, [HEADER] + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".h"))])
+
+
+def binding_stale():
+    return _stale(BINDING, [HEADER, os.path.join(CSRC, BINDING_SOURCE)])
+
+
 def needs_build():
-    if not os.path.exists(OUT) or not os.path.exists(BINDING):
-        return True
-    t = min(os.path.getmtime(OUT), os.path.getmtime(BINDING))
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
-    deps.append(os.path.join(os.path.dirname(os.path.dirname(HERE)), "include", "dsw_hip.h"))
-    return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
+    return library_stale() or binding_stale()
 
 
 def build_binding(verbose=True):
@@ -52,6 +62,9 @@ def build(force=False, verbose=True):
     """Compile every .hip translation unit for gfx950 (in parallel), link libdsw_hip.so, build the tensor binding."""
     if not force and not needs_build():
         return OUT
+    if not force and not library_stale():
+        build_binding(verbose)
+        return OUT
     from concurrent.futures import ThreadPoolExecutor
 
     objdir = os.path.join(CSRC, "obj")
@@ -71,9 +84,10 @@ def build(force=False, verbose=True):
         return obj
 
     with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
-        binding = ex.submit(build_binding, verbose)
+        binding = ex.submit(build_binding, verbose) if force or binding_stale() else None
         objs = list(ex.map(compile_one, SOURCES))
-        binding.result()
+        if binding is not None:
+            binding.result()
     cmd = [hipcc_path(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", OUT, *objs]
     if verbose:
         print("[dsw build]", " ".join(cmd), flush=True)

@@ -217,7 +217,7 @@ def test_quantize_weight(fin, fout, dtype):
 
 
 # (rows, K, N): one of everything; few rows; odd sizes; past one tile in each direction; long K; narrow and wide outputs
-MIX_SIZES = [(1, 1, 1), (1, 4096, 256), (2, 128, 16), (3, 100, 130), (16, 512, 64), (17, 1100, 33), (33, 640, 1000), (48, 2048, 96),
+MIX_SIZES = [(17, 128, 16), (31, 4096, 48), (63, 1040, 130), (100, 16, 33), (1, 1, 1), (1, 4096, 256), (2, 128, 16), (3, 100, 130), (16, 512, 64), (17, 1100, 33), (33, 640, 1000), (48, 2048, 96),
              (65, 127, 129), (64, 16, 8), (130, 129, 257), (200, 384, 512), (256, 256, 256), (300, 1000, 7), (517, 272, 384),
              (1000, 512, 128), (1, 20000, 40), (40, 9000, 24), (128, 8192, 160)]
 
@@ -281,8 +281,8 @@ def test_product(rows, K, N, dtype):
 
 
 # many rows: (rows, K, N, bytes behind a row), for the tiles of 128 x 128 and 256 x 256, whole and odd sizes in every direction
-TILE_SIZES = [(1030, 160, 1100, 0), (1024, 512, 1024, 0), (2001, 272, 515, 16), (1030, 301, 1100, 0), (1100, 1000, 1029, 7), (8200, 16, 129, 0),
-              (4100, 400, 4120, 0), (4096, 256, 4096, 0), (5000, 144, 4000, 112)]
+TILE_SIZES = [(700, 400, 70, 0), (1000, 1040, 97, 48), (6000, 256, 500, 0), (3000, 144, 60, 0), (1030, 160, 1100, 0), (1024, 512, 1024, 0), (2001, 272, 515, 16), (1030, 301, 1100, 0), (1100, 1000, 1029, 7), (8200, 16, 129, 0),
+              (4100, 784, 4120, 0), (4096, 768, 4096, 0), (5000, 144, 4000, 112), (4300, 900, 4001, 3)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -302,7 +302,7 @@ def test_product_of_many_rows(rows, K, N, gap, dtype):
     assert torch.equal(again, y)
 
 
-@pytest.mark.parametrize("rows", [1, 40, 300])
+@pytest.mark.parametrize("rows", [1, 20, 40, 300, 3000])
 def test_product_layouts(rows):
     """Slices of wider rows and weights at every byte alignment, leading axes, one scale for all rows, no rows."""
     K, N = 272, 150
