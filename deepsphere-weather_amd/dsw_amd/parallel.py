@@ -322,6 +322,19 @@ class GradBucket:
 
     __call__ = finish
 
+    def clip_norm(self, max_norm, norm_type=2.0):
+        """Scale the gradients by ``min(1, max_norm / (norm + 1e-6))`` with the norm (1, 2 or inf) of all of them taken together,
+        and return that norm (0-dim, on the device).  Call it after ``finish()``: the averaged gradients are the same on every
+        rank, so every rank derives the same factor and nothing is exchanged.  No host read: it may sit inside a captured step."""
+        from . import functional
+
+        if self.attached:
+            if any(p.grad is not self.views[p] for p in self.params):
+                raise RuntimeError("GradBucket: a parameter's gradient is no longer in the bucket (zero_grad(set_to_none=True)?); "
+                                   "zero() puts it back")
+            return functional.clip_grad_norm_(self.bucket, max_norm, norm_type)
+        return functional.clip_grad_norm_([p.grad for p in self.params if p.grad is not None], max_norm, norm_type)
+
     # ---- detached mode (gradients are ordinary tensors: copy in, exchange, copy out)
     def _pack(self):
         have = [p.grad is not None for p in self.params]

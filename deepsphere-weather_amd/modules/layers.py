@@ -434,6 +434,31 @@ def get_conv_fun(conv_type):
     return {"image": Conv2dEquiangular, "graph": ConvCheb}[conv_type]
 
 
+class RMSNorm(torch.nn.Module):
+    """Root-mean-square norm over the channels of every node of ``(sample, node, channel)`` tensors, an extension next to the
+    reference's ``BatchNorm1d`` option: it needs neither batch statistics (an autoregressive rollout has one sample) nor the two
+    transposes, and takes the residual's addition with it.
+
+    ``norm(x)`` -> y;  ``norm(x, residual)`` -> ``(y, x + residual)``;  ``norm.rows_fp8(x, residual)`` -> the same with y as
+    8-bit rows for :func:`dsw_amd.functional.dense_mix_fp8` (serving, under ``torch.no_grad()``)."""
+
+    def __init__(self, channels, eps=1e-6):
+        super().__init__()
+        self.channels, self.eps = int(channels), float(eps)
+        self.weight = torch.nn.Parameter(torch.ones(self.channels))
+
+    def extra_repr(self):
+        return f"{self.channels}, eps={self.eps}"
+
+    def forward(self, x, residual=None):
+        if residual is None:
+            return _F.rms_norm(x, self.weight, self.eps)
+        return _F.rms_norm_residual(x, residual, self.weight, self.eps)
+
+    def rows_fp8(self, x, residual=None):
+        return _F.rms_norm_fp8(x, self.weight, residual=residual, eps=self.eps)
+
+
 class GeneralConvBlock(ABC, torch.nn.Module):
     @abstractmethod
     def forward(self, *args, **kwargs):

@@ -98,6 +98,16 @@ class _NodeLinear(Linear):
         super().__init__(*args, **kwargs)
         self._lay_out_weight()
 
+    _fp8 = None          # (Fp8Weight, the weight's version it was made from) while the 8-bit path is on
+
+    def serve_fp8(self, enable=True):
+        """Inference through the 8-bit channel mix: the weight is quantised now (a scale per 128 x 128 block), the input rows
+        in each call.  Only calls under ``torch.no_grad()`` take it; moving or casting the module switches it off, and a weight
+        that has changed since raises (call it again)."""
+        with torch.no_grad():
+            self._fp8 = (dsw_functional.quantize_fp8_weight(self.weight.t()), self.weight._version) if enable else None
+        return self
+
     def _lay_out_weight(self):
         # only a REGISTERED parameter is re-laid, and only in place of its data: SWAG (reference modules/swag.py:33-48)
         # pops every entry of `_parameters` before `.to(device)` and later assigns plain tensors by attribute - there is
@@ -109,10 +119,16 @@ class _NodeLinear(Linear):
 
     def _apply(self, fn, *args, **kwargs):
         out = super()._apply(fn, *args, **kwargs)     # .to() / .cuda() keep dense strides; anything that did not is re-laid
+        self._fp8 = None
         self._lay_out_weight()
         return out
 
     def forward(self, x):
+        if self._fp8 is not None and not torch.is_grad_enabled():
+            weight, version = self._fp8
+            if self.weight._version != version:
+                raise RuntimeError("the weight has changed since serve_fp8(): call it again (or serve_fp8(False))")
+            return dsw_functional.dense_mix_fp8(x, weight, self.bias)
         # `weight.t()` is dense [in, out] for the column-major parameter; a row-major tensor (SWAG sample, user
         # assignment) is made contiguous inside dense_mix - same values either way
         # (the parameter's gradient buffer, if a GradBucket in direct mode attached one: memory order [in][out], which is
@@ -213,6 +229,15 @@ class ResBlock(torch.nn.Module):
             return dsw_functional.rezero_residual(y, self.res_connection(x), self.rezero_weight, out=out)
         y += self.res_connection(x)
         return y if out is None else out.copy_(y)
+
+
+def serve_fp8(model, enable=True):
+    """Switch the residual branches (``res_connection``) of ``model`` to the 8-bit channel mix for inference, or back; returns
+    how many there are.  The Chebyshev convolutions keep their precision."""
+    found = [m for m in model.modules() if isinstance(m, _NodeLinear)]
+    for m in found:
+        m.serve_fp8(enable)
+    return len(found)
 
 
 # (attribute, input width, output widths, level) of the six residual blocks; "in" / "out" stand for the model's

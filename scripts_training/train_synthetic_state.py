@@ -10,7 +10,8 @@ inspect-filtered kwargs convention -> ``.to(device)`` -> Adam(eps=1e-7) (``train
 -> ``WeightedMSELoss`` with the sampling's area weights (``:325-330``, ``modules/loss.py:118-156``) ->
 autoregressive steps: ``ar_iterations`` + 1 forwards per optimisation step, the prediction replacing the most
 recent dynamic features of the input window (``stack_most_recent_prediction``), the loss summed over the
-iterations, one backward, one flat-bucket gradient all-reduce when launched under torchrun, optimizer step.
+iterations, one backward, one flat-bucket gradient all-reduce when launched under torchrun, the clipping of the gradients by
+their global norm (``training_settings.max_grad_norm``; absent: none), optimizer step.
 The whole step (~77 ConvCheb launches x 7 forwards at the default config) is captured once into a HIP graph and
 replayed; under torchrun parameters and operator buffers are broadcast from rank 0 first (ARPACK's lambda_max
 estimate is not deterministic, so independently built replicas would not share one operator).
@@ -107,7 +108,8 @@ class Trainer:
     (``overlap``); with ``use_graph`` and N > 1 the graph holds forwards + backward, the chunks go out back to back after
     the replay and the optimizer update follows eagerly."""
 
-    def __init__(self, model, x, targets, n_dyn, lr, weights=None, stack=True, use_graph=True, dim_names=None):
+    def __init__(self, model, x, targets, n_dyn, lr, weights=None, stack=True, use_graph=True, dim_names=None,
+                 max_grad_norm=None):
         from dsw_amd.parallel import GradBucket
         from modules.loss import WeightedMSELoss
 
@@ -126,6 +128,8 @@ class Trainer:
         # themselves (no autograd `add` per use).  An eager N > 1 run keeps the hook-driven overlapped exchange instead.
         if x.is_cuda and (not self.distributed or use_graph):
             self.bucket.direct_accumulation()
+        self.max_grad_norm = max_grad_norm      # None: gradients are not clipped
+        self.grad_norm = None                   # norm before clipping of the last step (0-dim, on the device)
         self.loss = None
         self.graph = None
         self.sync_in_graph = False
@@ -139,10 +143,16 @@ class Trainer:
         loss.backward()
         return loss.detach()
 
+    def _update(self):
+        """Clip the (averaged) gradients by their common norm when asked to, then step the optimizer."""
+        if self.max_grad_norm is not None:
+            self.grad_norm = self.bucket.clip_norm(self.max_grad_norm)
+        self.optimizer.step()
+
     def _eager_step(self):
         loss = self._fwd_bwd()
         self.bucket.finish()
-        self.optimizer.step()
+        self._update()
         return loss
 
     def _capture(self):
@@ -171,7 +181,7 @@ class Trainer:
                 if self.sync_in_graph:
                     self.bucket.finish()      # all chunks back to back, as nodes of the graph
                 if not self.distributed or self.sync_in_graph:
-                    self.optimizer.step()
+                    self._update()
             self.bucket.capturing = False
             if not self.sync_in_graph:
                 self.bucket.finish()          # resets the hook counters of the recorded backward
@@ -213,7 +223,7 @@ class Trainer:
         self.graph.replay()
         if self.distributed and not self.sync_in_graph:
             self.bucket.finish()
-            self.optimizer.step()
+            self._update()
         return self.loss
 
 
@@ -249,7 +259,7 @@ def build_trainer(cfg, device, dtype=None, batch_size=None, ar_iterations=None, 
                for _ in range(n_ar)]
     trainer = Trainer(model, x, targets, n_dyn, ts.get("learning_rate", 0.007), weights=weights,
                       stack=ar.get("stack_most_recent_prediction", True), use_graph=use_graph,
-                      dim_names=info["dim_order"]["dynamic"])
+                      dim_names=info["dim_order"]["dynamic"], max_grad_norm=ts.get("max_grad_norm"))
     return trainer, {"B": B, "V": V, "n_ar": n_ar, "architecture": ms["architecture_name"],
                      "parameters": sum(p.numel() for p in model.parameters())}
 

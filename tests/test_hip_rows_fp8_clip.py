@@ -589,3 +589,132 @@ def test_captured_backward_refuses_leaves_of_a_living_graph():
     torch.cuda.synchronize()
     for a, b in zip(res, want):
         assert float((a - b).abs().max()) <= 1e-6 * float(b.abs().max())
+
+
+# ---- the framework's own paths -------------------------------------------------------------------------------------------
+def test_rms_norm_layer_in_a_bucket():
+    """The layer's gradients land in the flat bucket and are clipped there with the others, which feed the optimizer."""
+    from dsw_amd.parallel import FlatGradAllReduce, GradBucket
+    from modules.layers import RMSNorm
+    from modules.my_models_graph import _NodeLinear
+
+    torch.manual_seed(0)
+    norm, lin = RMSNorm(48).to(DEV), _NodeLinear(48, 20).to(DEV)
+    params = [*norm.parameters(), *lin.parameters()]
+    x, r = torch.randn(3, 50, 48, device=DEV), torch.randn(3, 50, 48, device=DEV)
+
+    def loss():
+        y, h = norm(x, r)
+        return (lin(y).square().sum() + h.sum())
+
+    plain = torch.autograd.grad(loss(), params)
+    want = math.sqrt(sum(float(g.double().square().sum()) for g in plain))
+    for bucket in (GradBucket(params, overlap=False), FlatGradAllReduce(params)):
+        if bucket.attached:
+            bucket.zero()
+        else:
+            for p in params:
+                p.grad = None
+        loss().backward()
+        bucket.finish()
+        n = bucket.clip_norm(1.0)
+        assert abs(float(n) - want) <= 1e-6 * want
+        for p, g in zip(params, plain):
+            assert float((p.grad - g / want).abs().max()) <= 2e-6 * float(g.abs().max()) / want
+        if bucket.attached:
+            bucket.detach()
+
+
+def test_residual_branch_in_8_bits():
+    """The node-wise Linear under serve_fp8 against 64 bits on its own e4m3 values; training and switching back are untouched."""
+    from modules.my_models_graph import _NodeLinear
+
+    torch.manual_seed(1)
+    lin = _NodeLinear(200, 72).to(DEV)
+    x = torch.randn(2, 90, 200, device=DEV)
+    with torch.no_grad():
+        plain = lin(x)
+        lin.serve_fp8()
+        y = lin(x)
+        rows, w8 = F.quantize_fp8(x), lin._fp8[0]
+        flat = rows.q.cpu().reshape(180, 200), rows.scale.cpu().reshape(180, 2), w8.q.cpu(), w8.scale.cpu()
+        want, mag = _mix64(*flat, lin.bias.detach().cpu())
+        _within(y.reshape(180, 72), want, _mix_tol(want, mag, 200, torch.float32), "y")
+        # each factor is off by 2^-4 of itself or 2^-10 of its scale, whichever is more; 1e-5 for the fp32 sums of both paths
+        a, b = x.double().reshape(180, 200).abs().cpu(), lin.weight.double().abs().cpu()
+        ea = torch.maximum(2.0 ** -4 * a, 2.0 ** -10 * flat[1].double().repeat_interleave(128, 1)[:, :200])
+        eb = torch.maximum(2.0 ** -4 * b, 2.0 ** -10 * flat[3].double().repeat_interleave(128, 1)[:, :200].expand_as(b))
+        _within(y.reshape(180, 72), plain.double().reshape(180, 72).cpu(), (a + ea) @ (b + eb).t() - a @ b.t() + 1e-5, "against the plain layer")
+        assert not torch.equal(y, plain)
+    assert torch.equal(lin(x), plain)                     # with gradients the layer is what it was
+    with torch.no_grad():
+        lin.weight.mul_(1.0)
+        with pytest.raises(RuntimeError, match="has changed"):
+            lin(x)
+        assert torch.equal(lin.serve_fp8(False)(x), plain)
+        lin.serve_fp8()
+        assert lin.to(torch.float32)._fp8 is None
+
+
+def _small_trainer(max_grad_norm, use_graph):
+    import json
+    import os
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    sys.path.insert(0, os.path.join(root, "scripts_training"))
+    import train_synthetic_state as drv
+
+    cfg = drv.read_config(os.path.join(root, "configs/UNetSpherical/Healpix_400km/InterpPool-Graph_knn.synthetic.json"))
+    cfg = json.loads(json.dumps(cfg))
+    cfg["model_settings"]["sampling_kwargs"]["subdivisions"] = 4
+    cfg["model_settings"]["knn"] = 8
+    if max_grad_norm is not None:
+        cfg["training_settings"]["max_grad_norm"] = max_grad_norm
+    return drv.build_trainer(cfg, torch.device(DEV), batch_size=2, ar_iterations=1, use_graph=use_graph)[0]
+
+
+def test_unet_serves_its_residual_branches_in_8_bits():
+    from modules.my_models_graph import serve_fp8
+
+    model = _small_trainer(None, False).model.eval()
+    x = torch.randn(2, 3, 192, 6, device=DEV)
+    with torch.no_grad():
+        plain = model(x)
+        assert serve_fp8(model) >= 4
+        y = model(x)
+        assert y.shape == plain.shape and bool(y.isfinite().all()) and not torch.equal(y, plain)
+        gr = torch.cuda.CUDAGraph()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            model(x)
+        torch.cuda.current_stream().wait_stream(side)
+        with torch.cuda.graph(gr):
+            out = model(x)
+        for _ in range(2):
+            gr.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, y)
+        serve_fp8(model, enable=False)
+        assert torch.equal(model(x), plain)
+
+
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_trainer_clips_by_the_global_norm(use_graph):
+    """training_settings.max_grad_norm: after a step the bucket holds gradients of that norm, captured or not; without it the
+    step is what it was."""
+    plain = _small_trainer(None, use_graph)
+    plain.step()
+    raw = plain.bucket.bucket.clone()
+    full = float(raw.double().norm())
+    t = _small_trainer(full / 4, use_graph)
+    assert t.grad_norm is None or use_graph
+    t.step()
+    torch.cuda.synchronize()
+    assert abs(float(t.grad_norm) - full) <= 1e-4 * full                    # (two builds of one model: fp32 steps in other orders)
+    assert abs(float(t.bucket.bucket.double().norm()) - full / 4) <= 1e-6 * full
+    assert float((t.bucket.bucket - raw / 4).abs().max()) <= 1e-4 * float(raw.abs().max())
+    wide = _small_trainer(full * 4, use_graph)
+    wide.step()
+    assert abs(float(wide.bucket.bucket.double().norm()) - full) <= 1e-4 * full

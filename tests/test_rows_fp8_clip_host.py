@@ -183,3 +183,34 @@ def test_rows_of_views():
     got, rows, step = as_rows(scale, True)
     assert got.data_ptr() == scale.data_ptr() and got.stride() == scale.stride() and (rows, step, got.stride(-1)) == (12, 1, 12)
     assert as_rows(torch.ones(1, 3).expand(12, 3), True)[2] == 0
+
+
+def test_layers_and_bucket_reach_the_operators():
+    from dsw_amd.parallel import FlatGradAllReduce, GradBucket
+    from modules.layers import RMSNorm
+    from modules.my_models_graph import _NodeLinear, serve_fp8
+
+    norm = RMSNorm(8, eps=1e-5)
+    assert [n for n, _ in norm.named_parameters()] == ["weight"] and bool((norm.weight == 1).all())
+    with passed():
+        norm(torch.randn(2, 3, 8))
+    with passed():
+        norm(torch.randn(2, 3, 8), torch.randn(2, 3, 8))
+    with passed(), torch.no_grad():
+        norm.rows_fp8(torch.randn(2, 3, 8))
+    lin = _NodeLinear(8, 4)
+    with passed():
+        lin.serve_fp8()
+    assert serve_fp8(torch.nn.Sequential(lin, torch.nn.ReLU()), enable=False) == 1
+    for bucket in (GradBucket([lin.weight, lin.bias]), FlatGradAllReduce([lin.weight, lin.bias])):
+        with passed():
+            if not bucket.attached:
+                lin.weight.grad = torch.ones_like(lin.weight)
+            bucket.clip_norm(1.0)
+    bucket = GradBucket([lin.weight, lin.bias])
+    lin.weight.grad = None
+    with pytest.raises(RuntimeError, match="no longer in the bucket"):
+        bucket.clip_norm(1.0)
+    with pytest.raises(ValueError, match="max_norm"):
+        bucket.zero()
+        bucket.clip_norm(-1.0)
