@@ -979,14 +979,18 @@ def _arm_watchdog(rank, world, limit=None, what="the run", retry=False):
         if retry and nxt is not None:
             # launched by somebody else's torchrun (the driver's scaling run): nobody will start a second attempt for us,
             # and a rank that exits takes the whole job down.  Every rank sits behind the same guard, so every rank
-            # replaces its own process image with the next, more conservative rung (same RANK / WORLD_SIZE / MASTER_*,
-            # a new process group behind its own store prefix - dsw_amd.parallel.init_from_env).
+            # runs the next, more conservative rung in its place (same RANK / WORLD_SIZE / MASTER_*, a new process group
+            # behind its own store prefix - dsw_amd.parallel.init_from_env): in a child, whose exit code becomes its own.
+            # (A process that has initialised the GPU may not be replaced by exec where the driver or a sandbox refuses it.)
             print("bench.py: rank %d/%d: %s still not finished after %.0f s - re-executing with %s" % (
                 rank, world, what, limit, nxt), file=sys.stderr, flush=True)
             env = dict(os.environ, **nxt)
             env["DSW_PG_ATTEMPT"] = str(int(os.environ.get("DSW_PG_ATTEMPT", "0") or 0) + 1)
             sys.stdout.flush()
-            os.execve(sys.executable, [sys.executable, os.path.abspath(__file__), *sys.argv[1:]], env)
+            import subprocess
+
+            rc = subprocess.call([sys.executable, os.path.abspath(__file__), *sys.argv[1:]], env=env)
+            os._exit(rc if rc >= 0 else 128 - rc)
         print("bench.py: rank %d/%d: %s still not finished after %.0f s - giving up" % (rank, world, what, limit),
               file=sys.stderr, flush=True)
         os._exit(124)
