@@ -352,13 +352,15 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
     store_tile<NT, MT, BF16, WAVES * NT * MT >= 256>(P, acc, lds + wave * OWN, n0 + wn, m0 + wm, lane);
 }
 
-// rows of any alignment and length -> rows of whole 16-byte chunks, zero behind the row; then the kernels above take them
-__global__ __launch_bounds__(256) void fp8_align_rows_kernel(const uint8_t* X, long ld, int K, uint8_t* out, long rows, int chunks) {
+// rows of any alignment and length (M of X, then N of W) -> rows of whole 16-byte chunks, zero behind the row; then the kernels
+// above take them
+__global__ __launch_bounds__(256) void fp8_align_rows_kernel(const uint8_t* X, long ldx, const uint8_t* W, long ldw, int K, uint8_t* out, long M,
+                                                             long rows, int chunks) {
     const long total = rows * chunks;
     for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long)gridDim.x * 256) {
         const long r = e / chunks;
         const int c = (int)(e - r * chunks);
-        reinterpret_cast<u32x4*>(out)[e] = row_chunk(X + r * ld, c * 16, K);
+        reinterpret_cast<u32x4*>(out)[e] = row_chunk(r < M ? X + r * ldx : W + (r - M) * ldw, c * 16, K);
     }
 }
 
@@ -633,10 +635,10 @@ static int launch_mix(const MixArgs& a, hipStream_t s) {
     return launch_tile<2, 2, 1, 4, BF16>(a, s);
 }
 
-static int align_rows(const uint8_t* X, long ld, int K, uint8_t* out, long rows, hipStream_t s) {
-    const int chunks = (K + 15) / 16;
-    const long blocks = (rows * chunks + 255) / 256;
-    DSW_LAUNCH(fp8_align_rows_kernel, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, X, ld, K, out, rows, chunks);
+static int align_rows(const MixArgs& a, uint8_t* out, hipStream_t s) {
+    const int chunks = (a.K + 15) / 16;
+    const long rows = (long)a.M + a.N, blocks = (rows * chunks + 255) / 256;
+    DSW_LAUNCH(fp8_align_rows_kernel, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, a.X, a.ldx, a.W, a.ldw, a.K, out, (long)a.M, rows, chunks);
     return dsw_check_launch();
 }
 
@@ -671,8 +673,7 @@ int dsw_fp8_mix(const void* X, int64_t ldx, const float* XS, int64_t xs_row, int
         const long ld = (long)((K + 15) / 16 * 16);
         uint8_t* const x = static_cast<uint8_t*>(workspace);
         uint8_t* const w = x + M * ld;
-        int rc = align_rows(a.X, a.ldx, a.K, x, (long)M, s);
-        if (rc == DSW_OK) rc = align_rows(a.W, a.ldw, a.K, w, (long)N, s);
+        const int rc = align_rows(a, x, s);
         if (rc != DSW_OK) return rc;
         a.X = x; a.W = w; a.ldx = a.ldw = ld; a.K = (int)ld;       // (zeros behind the rows; the same number of scale blocks)
     }

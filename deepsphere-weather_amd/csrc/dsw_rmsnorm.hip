@@ -5,7 +5,9 @@
 //     dx = dr = D + rstd (G w - xhat mean_c(G w xhat)),     dw = sum over rows of G xhat
 // All of it is bound by HBM: a row is read once into registers (16 bytes per lane and access), the sums run over the lanes that
 // share the row, and everything that a pass can derive from the row leaves in the same pass.  The square sum and the norm use
-// the unrounded fp32 sum x + r; h itself is rounded to the storage type once, and it is what the backward pass reads again.
+// the unrounded fp32 sum x + r; h itself is rounded to the storage type once.  The backward pass takes the two addends rather than
+// the rounded h: with bf16 storage the rounding would be as large an error in dw as dw's own (1.5 x together; a fifth stream
+// read, 10 us of 84 at 98304 x 256).
 #include "dsw_rows_common.h"
 #include "../../include/dsw_hip.h"
 
@@ -184,9 +186,9 @@ __global__ __launch_bounds__(RN_THREADS) void rmsnorm_fwd_long_kernel(const Norm
 }
 
 struct NormBwdArgs {
-    const char* G; const char* D; const char* H; const char* W; const float* rstd;
+    const char* G; const char* D; const char* X; const char* R; const char* W; const float* rstd;
     char* dX; float* part;      // part: [blocks][C] column sums, or null when dw is not asked for
-    long rows, ldh;
+    long rows, ldx, ldr;
     int C;
 };
 
@@ -221,8 +223,14 @@ __global__ __launch_bounds__(RN_THREADS) void rmsnorm_bwd_kernel(const NormBwdAr
 #pragma unroll
             for (int j = 0; j < V; ++j) h[i][j] = g[i][j] = 0.f;
             if (n > 0) {
-                Rw::load(P.H + (row * P.ldh + c) * E, n, h[i]);
+                Rw::load(P.X + (row * P.ldx + c) * E, n, h[i]);
                 Rw::load(P.G + (row * P.C + c) * E, n, g[i]);
+                if (P.R != nullptr) {
+                    float r[V];
+                    Rw::load(P.R + (row * P.ldr + c) * E, n, r);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) h[i][j] += r[j];
+                }
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) {
@@ -279,11 +287,20 @@ __global__ __launch_bounds__(RN_THREADS) void rmsnorm_bwd_long_dx_kernel(const N
     __shared__ float red[2][4];
     int flip = 0;
     for (long row = blockIdx.x; row < P.rows; row += gridDim.x, flip ^= 1) {
+    auto stream = [&](int c, float (&h)[V]) {
+        Rw::load(P.X + (row * P.ldx + c) * E, P.C - c, h);
+        if (P.R != nullptr) {
+            float r[V];
+            Rw::load(P.R + (row * P.ldr + c) * E, P.C - c, r);
+#pragma unroll
+            for (int j = 0; j < V; ++j) h[j] += r[j];
+        }
+    };
     const float rstd = P.rstd[row];
     float a = 0.f;
     for (int c = threadIdx.x * V; c < P.C; c += RN_THREADS * V) {
         float h[V], g[V], w[V];
-        Rw::load(P.H + (row * P.ldh + c) * E, P.C - c, h);
+        stream(c, h);
         Rw::load(P.G + (row * P.C + c) * E, P.C - c, g);
         Rw::load(P.W + (long)c * E, P.C - c, w);
 #pragma unroll
@@ -292,7 +309,7 @@ __global__ __launch_bounds__(RN_THREADS) void rmsnorm_bwd_long_dx_kernel(const N
     a = row_sum<RN_THREADS>(a, red, flip) / (float)P.C;
     for (int c = threadIdx.x * V; c < P.C; c += RN_THREADS * V) {
         float h[V], g[V], w[V], d[V];
-        Rw::load(P.H + (row * P.ldh + c) * E, P.C - c, h);
+        stream(c, h);
         Rw::load(P.G + (row * P.C + c) * E, P.C - c, g);
         Rw::load(P.W + (long)c * E, P.C - c, w);
 #pragma unroll
@@ -312,7 +329,8 @@ __global__ __launch_bounds__(RN_THREADS) void rmsnorm_bwd_long_dw_kernel(const N
     if (c >= P.C) return;
     float s = 0.f;
     for (long row = blockIdx.y; row < P.rows; row += gridDim.y)
-        s = fmaf(Rw::one(P.G + (row * P.C + c) * E), Rw::one(P.H + (row * P.ldh + c) * E) * P.rstd[row], s);
+        s = fmaf(Rw::one(P.G + (row * P.C + c) * E),
+                 (Rw::one(P.X + (row * P.ldx + c) * E) + (P.R != nullptr ? Rw::one(P.R + (row * P.ldr + c) * E) : 0.f)) * P.rstd[row], s);
     P.part[(long)blockIdx.y * P.C + c] = s;
 }
 
@@ -512,17 +530,17 @@ int64_t dsw_rmsnorm_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype) {
     return bwd_blocks(rows, C, dtype) * C * 4;
 }
 
-int dsw_rmsnorm_bwd(const void* G, const void* D, const void* H, int64_t ldh, const void* W, const float* rstd, void* dX, void* dW,
+int dsw_rmsnorm_bwd(const void* G, const void* D, const void* X, int64_t ldx, const void* R, int64_t ldr, const void* W, const float* rstd, void* dX, void* dW,
                     void* workspace, int64_t workspace_bytes, int64_t rows, int64_t C, int dtype, dsw_stream_t stream) {
     if (!dtype_ok(dtype)) return DSW_ERR_BAD_DTYPE;
-    if (!rows_ok(rows, C) || ldh < C || !W || (!dX && !dW)) return DSW_ERR_BAD_ARG;
-    if (rows > 0 && (!G || !H || !rstd)) return DSW_ERR_BAD_ARG;
+    if (!rows_ok(rows, C) || ldx < C || (R && ldr < C) || !W || (!dX && !dW)) return DSW_ERR_BAD_ARG;
+    if (rows > 0 && (!G || !X || !rstd)) return DSW_ERR_BAD_ARG;
     if (dW && (!workspace || workspace_bytes < dsw_rmsnorm_bwd_workspace_bytes(rows, C, dtype))) return DSW_ERR_WORKSPACE;
     if (rows == 0 && !dW) return DSW_OK;
     hipStream_t s = (hipStream_t)stream;
     DswTraceScope trace_(s, DSW_ROLE_RMSNORM, rows, C, 4);
-    const NormBwdArgs a{(const char*)G, (const char*)D, (const char*)H, (const char*)W, rstd, (char*)dX,
-                        dW ? (float*)workspace : nullptr, (long)rows, (long)ldh, (int)C};
+    const NormBwdArgs a{(const char*)G, (const char*)D, (const char*)X, (const char*)R, (const char*)W, rstd, (char*)dX,
+                        dW ? (float*)workspace : nullptr, (long)rows, (long)ldx, (long)ldr, (int)C};
     return dtype == DSW_BF16 ? launch_bwd<true>(a, (char*)dW, s) : launch_bwd<false>(a, (char*)dW, s);
 }
 

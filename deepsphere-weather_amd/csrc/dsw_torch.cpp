@@ -121,7 +121,7 @@ void check_norm(const Tensor& x, const Tensor& r, const Tensor& w, double eps) {
     if (r.defined()) { same_type(x, r); same_device(x, r); }
 }
 
-struct NormOut { Tensor y, h, rstd, saved; };
+struct NormOut { Tensor y, h, rstd, x, r; };        // x, r: the rows as the kernel read them
 NormOut norm_forward(const Tensor& x, const Tensor& r, const Tensor& w, double eps, bool need_rstd) {
     const c10::DeviceGuard guard(x.device());
     const Rows xr = as_rows(x);
@@ -131,7 +131,8 @@ NormOut norm_forward(const Tensor& x, const Tensor& r, const Tensor& w, double e
     if (need_rstd) o.rstd = at::empty({xr.rows}, x.options().dtype(at::kFloat));
     Rows rr{Tensor(), 0, 0};
     if (r.defined()) { rr = as_rows(r); o.h = at::empty(x.sizes(), x.options()); }
-    o.saved = r.defined() ? o.h : xr.t;
+    o.x = xr.t;
+    o.r = rr.t;
     check(lib.rmsnorm_fwd(xr.t.data_ptr(), xr.step, r.defined() ? rr.t.data_ptr() : nullptr, rr.step, wc.data_ptr(), o.y.data_ptr(),
                           r.defined() ? o.h.data_ptr() : nullptr, need_rstd ? o.rstd.data_ptr<float>() : nullptr, xr.rows, w.size(0),
                           (float)eps, code_of(x.scalar_type()), stream_of(x)), "dsw_rmsnorm_fwd");
@@ -168,31 +169,30 @@ variable_list once(variable_list grads) {
 }
 
 // {dx (of both addends), dw}
-std::array<Tensor, 2> norm_backward(AutogradContext* ctx, const Tensor& dy, const Tensor& dh, bool need_x, bool need_w) {
-    const auto saved = ctx->get_saved_variables();
-    const Tensor &h = saved[0], &w = saved[1], &rstd = saved[2];
+std::array<Tensor, 2> norm_backward(const Tensor& x, const Tensor& r, const Tensor& w, const Tensor& rstd, const Tensor& dy, const Tensor& dh,
+                                    bool need_x, bool need_w) {
     const at::AutoGradMode off(false);
-    refuse_foreign_leaves(h);
+    refuse_foreign_leaves(x);
     if (!dy.defined())                                // nothing behind y: the stream's own gradient passes through
         return {need_x ? dh : Tensor(), need_w ? at::zeros_like(w) : Tensor()};
-    const c10::DeviceGuard guard(h.device());
-    const Rows hr = as_rows(h);
+    const c10::DeviceGuard guard(x.device());
+    const Rows xr = as_rows(x), rr = r.defined() ? as_rows(r) : Rows{Tensor(), 0, 0};
     const Tensor g = dy.contiguous(), d = dh.defined() ? dh.contiguous() : dh;
-    const int code = code_of(h.scalar_type());
+    const int code = code_of(x.scalar_type());
     const int64_t C = w.size(0);
     Tensor dx, dw, ws;
     int64_t bytes = 0;
-    if (need_x) dx = at::empty(h.sizes(), h.options());
+    if (need_x) dx = at::empty(x.sizes(), x.options());
     if (need_w) {
         dw = at::empty(w.sizes(), w.options());
-        bytes = lib.rmsnorm_bwd_workspace_bytes(hr.rows, C, code);
+        bytes = lib.rmsnorm_bwd_workspace_bytes(xr.rows, C, code);
         check(bytes, "dsw_rmsnorm_bwd_workspace_bytes");
-        ws = at::empty({bytes}, h.options().dtype(at::kByte));
+        ws = at::empty({bytes}, x.options().dtype(at::kByte));
     }
     if (need_x || need_w)
-        check(lib.rmsnorm_bwd(g.data_ptr(), d.defined() ? d.data_ptr() : nullptr, hr.t.data_ptr(), hr.step, w.data_ptr(), rstd.data_ptr<float>(),
-                              need_x ? dx.data_ptr() : nullptr, need_w ? dw.data_ptr() : nullptr, need_w ? ws.data_ptr() : nullptr, bytes,
-                              hr.rows, C, code, stream_of(h)), "dsw_rmsnorm_bwd");
+        check(lib.rmsnorm_bwd(g.data_ptr(), d.defined() ? d.data_ptr() : nullptr, xr.t.data_ptr(), xr.step, r.defined() ? rr.t.data_ptr() : nullptr,
+                              rr.step, w.data_ptr(), rstd.data_ptr<float>(), need_x ? dx.data_ptr() : nullptr, need_w ? dw.data_ptr() : nullptr,
+                              need_w ? ws.data_ptr() : nullptr, bytes, xr.rows, C, code, stream_of(x)), "dsw_rmsnorm_bwd");
     return {dx, dw};
 }
 
@@ -200,28 +200,32 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, double eps) {
         const NormOut o = norm_forward(x, Tensor(), w, eps, true);
         ctx->set_materialize_grads(false);
-        ctx->save_for_backward({o.saved, w.contiguous(), o.rstd});
+        ctx->save_for_backward({o.x, w.contiguous(), o.rstd});
         return o.y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
-        const auto g = norm_backward(ctx, grads[0], Tensor(), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+        const auto saved = ctx->get_saved_variables();
+        const auto g = norm_backward(saved[0], Tensor(), saved[1], saved[2], grads[0], Tensor(), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
         return once({g[0], g[1], Tensor()});
     }
 };
 
-// with a residual the stored stream h is read again by backward (it is alive anyway: the next block's input)
+// bf16: backward reads both addends again (the stored stream h is their rounded sum, which dw would show); fp32: it reads h, which
+// is alive anyway as the next block's input
 struct RmsNormResidual : torch::autograd::Function<RmsNormResidual> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& r, const Tensor& w, double eps) {
         const NormOut o = norm_forward(x, r, w, eps, true);
         ctx->set_materialize_grads(false);
-        ctx->save_for_backward({o.h, w.contiguous(), o.rstd});
+        const bool both = x.scalar_type() == at::kBFloat16;
+        ctx->save_for_backward({both ? o.x : o.h, w.contiguous(), o.rstd, both ? o.r : Tensor()});
         return {o.y, o.h};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
         const bool need_x = ctx->needs_input_grad(0), need_r = ctx->needs_input_grad(1);
-        const auto g = norm_backward(ctx, grads[0], grads[1], need_x || need_r, ctx->needs_input_grad(2));
+        const auto saved = ctx->get_saved_variables();
+        const auto g = norm_backward(saved[0], saved[3], saved[1], saved[2], grads[0], grads[1], need_x || need_r, ctx->needs_input_grad(2));
         return once({need_x ? g[0] : Tensor(), need_r ? g[0] : Tensor(), g[1], Tensor()});
     }
 };

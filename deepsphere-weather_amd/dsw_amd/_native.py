@@ -108,7 +108,7 @@ SIGNATURES = {
     "dsw_quant_fp8": (_int, [_vp, _i64, _vp, _f32p, _i64, _i64, _i64, _int, _vp]),
     "dsw_quant_fp8_weight": (_int, [_vp, _i64, _i64, _vp, _f32p, _i64, _i64, _int, _vp]),
     "dsw_rmsnorm_bwd_workspace_bytes": (_i64, [_i64, _i64, _int]),
-    "dsw_rmsnorm_bwd": (_int, [_vp, _vp, _vp, _i64, _vp, _f32p, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
+    "dsw_rmsnorm_bwd": (_int, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _f32p, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
     "dsw_fp8_mix_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
     "dsw_fp8_mix": (_int, [_vp, _i64, _f32p, _i64, _i64, _vp, _i64, _f32p, _vp, _vp, _i64, _i64, _i64, _int, _vp, _i64, _vp]),
     "dsw_grad_norm_workspace_bytes": (_i64, []),

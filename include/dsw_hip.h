@@ -430,13 +430,13 @@ int dsw_quant_fp8(const void* X, int64_t ldx, void* Q, float* S, int64_t s_ld, i
 int dsw_quant_fp8_weight(const void* W, int64_t stride_in, int64_t stride_out, void* Q, float* S, int64_t Fin, int64_t Fout,
                          int dtype, dsw_stream_t stream);
 
-/* Backward of dsw_rmsnorm_fwd.  G = dL/dy, D = dL/dh or NULL, H = what the forward stored (or its input where there was no
- * residual; rows ldh elements apart), rstd as stored:
+/* Backward of dsw_rmsnorm_fwd.  G = dL/dy, D = dL/dh or NULL, X and R as the forward took them (R NULL without a residual; the
+ * stored H may stand for the sum: X = H, R = NULL, at the price of its rounding in dW), rstd as stored:
  *     dX = D + rstd (G w - xhat mean_c(G w xhat)),  xhat = h rstd     (the gradient of x AND of r);     dW = sum_rows G xhat
  * dX or dW may be NULL.  G, D, dX dense.  The workspace (dsw_rmsnorm_bwd_workspace_bytes) is needed for dW; no atomics: equal
  * inputs give equal bits.  rows == 0: dW = 0. */
 int64_t dsw_rmsnorm_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype);
-int dsw_rmsnorm_bwd(const void* G, const void* D, const void* H, int64_t ldh, const void* W, const float* rstd, void* dX, void* dW,
+int dsw_rmsnorm_bwd(const void* G, const void* D, const void* X, int64_t ldx, const void* R, int64_t ldr, const void* W, const float* rstd, void* dX, void* dW,
                     void* workspace, int64_t workspace_bytes, int64_t rows, int64_t C, int dtype, dsw_stream_t stream);
 
 /* Per-node linear map of e4m3 rows and e4m3 weights, a scale per block of 128:

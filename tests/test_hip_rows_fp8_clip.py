@@ -77,13 +77,11 @@ def test_norm_forward_and_backward(rows, C, residual, dtype):
     xhat, gw = h64 * rstd, dy.double() * w.double()
     a, mag = (gw * xhat).mean(-1, keepdim=True), (gw * xhat).abs().mean(-1, keepdim=True)
     want = rstd * (gw - xhat * a) + (dh.double() if residual else 0.0)
-    stored = HALF[dtype] if residual else 0.0        # backward reads h as it was stored: half a step of its type in xhat
-    tol = (HALF[dtype] + 2 * U) * want.abs() + 2 * n * U * rstd * (gw.abs() + xhat.abs() * mag) + 2 * U * (dh.double().abs() if residual else 0.0) \
-        + 2.2 * stored * rstd * xhat.abs() * mag
+    tol = (HALF[dtype] + 2 * U) * want.abs() + 2 * n * U * rstd * (gw.abs() + xhat.abs() * mag) + 2 * U * (dh.double().abs() if residual else 0.0)
     _within(dx, want, tol, "dx")
     dw64, dmag = (dy.double() * xhat).sum(0), (dy.double() * xhat).abs().sum(0)
     # dw: xhat (n / 2 + 6), rows of one chain, 16 groups, 128 partials of one chain, 8 joins
-    _within(dw, dw64, (HALF[dtype] + U) * dw64.abs() + ((n / 2 + 160 + rows / 1024) * U + 1.1 * stored) * dmag, "dw")
+    _within(dw, dw64, (HALF[dtype] + U) * dw64.abs() + (n / 2 + 160 + rows / 1024) * U * dmag, "dw")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -130,8 +130,9 @@ def test_c_entries_refuse_before_they_launch():
     need = lib.dsw_rmsnorm_bwd_workspace_bytes(1000, 256, 1)
     assert need > 0 and need % (256 * 4) == 0
     assert lib.dsw_rmsnorm_bwd_workspace_bytes(1000, 256, 3) == -2
-    assert lib.dsw_rmsnorm_bwd(p, None, p, 256, p, p, p, p, p, need - 1, 1000, 256, 1, None) == -3
-    assert lib.dsw_rmsnorm_bwd(p, None, p, 256, p, p, None, None, p, need, 1000, 256, 1, None) == -1
+    assert lib.dsw_rmsnorm_bwd(p, None, p, 256, None, 0, p, p, p, p, p, need - 1, 1000, 256, 1, None) == -3
+    assert lib.dsw_rmsnorm_bwd(p, None, p, 256, None, 0, p, p, None, None, p, need, 1000, 256, 1, None) == -1
+    assert lib.dsw_rmsnorm_bwd(p, None, p, 256, p, 255, p, p, p, p, p, need, 1000, 256, 1, None) == -1
     assert lib.dsw_fp8_mix_workspace_bytes(-1, 8, 8, 1) == -1
     assert lib.dsw_fp8_mix_workspace_bytes(1000, 8, 20, 1) == 0 and lib.dsw_fp8_mix_workspace_bytes(1000, 8, 20, 0) == 1008 * 32
     assert lib.dsw_fp8_mix(p, 20, p, 1, 1, p, 20, p, None, p, 1000, 8, 20, 0, p, 100, None) == -3
