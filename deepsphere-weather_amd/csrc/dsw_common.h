@@ -32,6 +32,13 @@ static __device__ __forceinline__ uint16_t f32_to_bf16(float f) {
     return (uint16_t)(u >> 16);
 }
 
+// two values to bf16, to nearest even, the first in the low half: one instruction of gfx950 (f32_to_bf16 is seven)
+static __device__ __forceinline__ uint32_t f32x2_to_bf16(float lo, float hi) {
+    typedef __attribute__((ext_vector_type(2))) float f32x2;
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
+}
+
 // Diagnostic switches (A/B runs, ablations, kernel-selection overrides) exist only in builds made with -DDSW_DIAG
 // (`DSW_BUILD_DIAG=1 python -m dsw_amd.build`): the product library reads NO environment variable - a process-wide,
 // read-once switch that silently changes the evaluation order has no place in it.

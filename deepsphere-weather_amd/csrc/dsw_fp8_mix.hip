@@ -160,7 +160,7 @@ static __device__ __forceinline__ void store_tile(const MixArgs& P, const f32x4 
             for (int q = 0; q < 4; ++q) {
                 if constexpr (BF16) {
                     const int e = c * 8 + 2 * q;
-                    v[q] = f32_to_bf16(acc[e / 4][j][e % 4] + add[e]) | (uint32_t)f32_to_bf16(acc[e / 4][j][e % 4 + 1] + add[e + 1]) << 16;
+                    v[q] = f32x2_to_bf16(acc[e / 4][j][e % 4] + add[e], acc[e / 4][j][e % 4 + 1] + add[e + 1]);
                 } else {
                     v[q] = __float_as_uint(acc[c][j][q] + add[4 * c + q]);
                 }

@@ -20,6 +20,10 @@ constexpr int GN_CHUNK = 256 * 32;         // elements of a workgroup's step: 4 
 constexpr int GN_BLOCKS = 1024;            // partial sums of one launch at most
 constexpr int GN_MAX_PARTS = 16 * 1024;    // partial sums of one call at most
 
+// from here on the results leave past the caches, which keep what the first pass read last for the second, going backwards
+// (200 M gradients, 500 MB: 281 us against 314; 7 MB: no difference)
+constexpr int64_t GN_STREAM_BYTES = (int64_t)128 << 20;
+
 struct GradTable {
     const char* g[GN_TENSORS];
     char* o[GN_TENSORS];
@@ -107,7 +111,7 @@ static __device__ __forceinline__ double total_norm(const double* part, int npar
     return P == GN_L2 ? sqrt(s) : s;
 }
 
-template <bool BF16>
+template <bool BF16, bool STREAM>
 static __device__ __forceinline__ void chunk_scale(const char* g, char* o, int n, float c) {
     using Rw = Row<BF16>;
     constexpr int V = Rw::V;
@@ -122,7 +126,8 @@ static __device__ __forceinline__ void chunk_scale(const char* g, char* o, int n
             Rw::unpack(t[q], v);
 #pragma unroll
             for (int j = 0; j < V; ++j) v[j] *= c;
-            Rw::put_raw(o + (long)(i + q * GN_THREADS * V) * Rw::E, Rw::pack(v));
+            if constexpr (STREAM) Rw::put_raw_stream(o + (long)(i + q * GN_THREADS * V) * Rw::E, Rw::pack(v));
+            else Rw::put_raw(o + (long)(i + q * GN_THREADS * V) * Rw::E, Rw::pack(v));
         }
     }
     for (; i < n; i += GN_THREADS * V) {
@@ -135,7 +140,7 @@ static __device__ __forceinline__ void chunk_scale(const char* g, char* o, int n
 }
 
 // T.n == 0: the norm alone
-template <int P>
+template <int P, bool STREAM>
 __global__ __launch_bounds__(GN_THREADS) void grad_clip_kernel(const GradTable T, const double* part, int nparts, double max_norm,
                                                                float* norm) {
     __shared__ double red[4];
@@ -144,14 +149,15 @@ __global__ __launch_bounds__(GN_THREADS) void grad_clip_kernel(const GradTable T
     if (T.n == 0) return;
     const double q = max_norm / (N + 1e-6);
     const float c = q > 1.0 ? 1.f : (float)q;                  // (a NaN stays one, as in max_norm / norm clamped from above)
-    for (long chunk = blockIdx.x; chunk < T.first[T.n]; chunk += gridDim.x) {
+    for (long at_ = blockIdx.x; at_ < T.first[T.n]; at_ += gridDim.x) {
+        const long chunk = T.first[T.n] - 1 - at_;             // from the end: what the first pass read last is still in the caches
         const int t = segment_of(T, chunk);
         if (c == 1.f && T.g[t] == T.o[t]) continue;            // in place and nothing to clip: g * 1 is g
         const long at = (chunk - T.first[t]) * GN_CHUNK;
         const int n = chunk + 1 == T.first[t + 1] ? T.tail[t] + 1 : GN_CHUNK;
         const bool bf16 = T.bf16[t >> 5] >> (t & 31) & 1u;
-        if (bf16) chunk_scale<true>(T.g[t] + at * 2, T.o[t] + at * 2, n, c);
-        else chunk_scale<false>(T.g[t] + at * 4, T.o[t] + at * 4, n, c);
+        if (bf16) chunk_scale<true, STREAM>(T.g[t] + at * 2, T.o[t] + at * 2, n, c);
+        else chunk_scale<false, STREAM>(T.g[t] + at * 4, T.o[t] + at * 4, n, c);
     }
 }
 
@@ -218,14 +224,19 @@ static int run_clip(const Piece* pieces, int64_t k, double* part, double max_nor
     }
     if (!scale || batches == 0) {
         T.n = 0;
-        DSW_LAUNCH(grad_clip_kernel<P>, dim3(1), dim3(GN_THREADS), 0, s, T, part, nparts, max_norm, norm);
+        DSW_LAUNCH((grad_clip_kernel<P, false>), dim3(1), dim3(GN_THREADS), 0, s, T, part, nparts, max_norm, norm);
         return dsw_check_launch();
     }
-    for (int b = 0; b < batches; ++b) {
+    int64_t bytes = 0;
+    for (int64_t i = 0; i < k; ++i) bytes += pieces[i].n * (pieces[i].bf16 ? 2 : 4);
+    const bool stream = bytes >= GN_STREAM_BYTES;
+    for (int b = batches - 1; b >= 0; --b) {
         const int64_t at = (int64_t)b * GN_TENSORS;
         fill_table(T, pieces + at, (int)(k - at < GN_TENSORS ? k - at : GN_TENSORS));
-        const int blocks = (int)(T.first[T.n] < 2048 ? T.first[T.n] : 2048);
-        DSW_LAUNCH(grad_clip_kernel<P>, dim3(blocks), dim3(GN_THREADS), 0, s, T, part, nparts, max_norm, b == 0 ? norm : nullptr);
+        const int blocks = (int)(T.first[T.n] < 2 * GN_BLOCKS ? T.first[T.n] : 2 * GN_BLOCKS);
+        float* const to = b == 0 ? norm : nullptr;
+        if (stream) DSW_LAUNCH((grad_clip_kernel<P, true>), dim3(blocks), dim3(GN_THREADS), 0, s, T, part, nparts, max_norm, to);
+        else DSW_LAUNCH((grad_clip_kernel<P, false>), dim3(blocks), dim3(GN_THREADS), 0, s, T, part, nparts, max_norm, to);
     }
     return dsw_check_launch();
 }

@@ -194,49 +194,71 @@ struct NormBwdArgs {
 
 // Every workgroup walks rows blockIdx.x, + gridDim.x, ... (in groups of 256 / TPR) and keeps its columns' share of dw in
 // registers; the groups of a workgroup join theirs in index order through LDS, the workgroups leave one row each in `part`.
-// No atomics: the order of every sum is fixed by the shape.
+// No atomics: the order of every sum is fixed by the shape.  The streams of a group's next row are on their way while it works on
+// the present one.
 template <bool BF16, int TPR, int NV>
 __global__ __launch_bounds__(RN_THREADS) void rmsnorm_bwd_kernel(const NormBwdArgs P) {
     using Rw = Row<BF16>;
+    using u32x4 = typename Rw::u32x4;
     constexpr int V = Rw::V, E = Rw::E, GROUPS = RN_THREADS / TPR;
     __shared__ float red[2][4];
     __shared__ float cols[GROUPS > 1 ? GROUPS * TPR * V : 1];
     const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
-    float w[NV][V], dw[NV][V];
+    float dw[NV][V];
+    u32x4 w[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * TPR) * V, n = P.C - c;
+        const int c = (t + i * TPR) * V;
+        w[i] = Rw::fetch(P.W + (long)c * E, P.C - c);
 #pragma unroll
-        for (int j = 0; j < V; ++j) w[i][j] = dw[i][j] = 0.f;
-        if (n > 0) Rw::load(P.W + (long)c * E, n, w[i]);
+        for (int j = 0; j < V; ++j) dw[i][j] = 0.f;
     }
-    int flip = 0;
-    for (long r0 = (long)blockIdx.x * GROUPS; r0 < P.rows; r0 += (long)gridDim.x * GROUPS) {
-        const long row = r0 + group;
+    u32x4 nx[NV], nr[NV], ng[NV], nd[NV];
+    float nrstd = 0.f;
+    auto ahead = [&](long row) {
         const bool live = row < P.rows;
-        const float rstd = live ? P.rstd[row] : 0.f;
-        float h[NV][V], g[NV][V];
-        float a = 0.f;
+        nrstd = live ? P.rstd[row] : 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (t + i * TPR) * V, n = live ? P.C - c : 0;
+            nx[i] = Rw::fetch(P.X + (row * P.ldx + c) * E, n);
+            ng[i] = Rw::fetch(P.G + (row * P.C + c) * E, n);
+            if (P.R != nullptr) nr[i] = Rw::fetch(P.R + (row * P.ldr + c) * E, n);
+            if (P.D != nullptr && P.dX != nullptr) nd[i] = Rw::fetch(P.D + (row * P.C + c) * E, n);
+        }
+    };
+    int flip = 0;
+    const long stride = (long)gridDim.x * GROUPS;
+    ahead((long)blockIdx.x * GROUPS + group);
+    for (long r0 = (long)blockIdx.x * GROUPS; r0 < P.rows; r0 += stride) {
+        const long row = r0 + group;
+        const bool live = row < P.rows;
+        const float rstd = nrstd;
+        float h[NV][V], g[NV][V];
+        u32x4 d[NV];
+        float a = 0.f;
 #pragma unroll
-            for (int j = 0; j < V; ++j) h[i][j] = g[i][j] = 0.f;
-            if (n > 0) {
-                Rw::load(P.X + (row * P.ldx + c) * E, n, h[i]);
-                Rw::load(P.G + (row * P.C + c) * E, n, g[i]);
-                if (P.R != nullptr) {
-                    float r[V];
-                    Rw::load(P.R + (row * P.ldr + c) * E, n, r);
+        for (int i = 0; i < NV; ++i) {
+            Rw::unpack(nx[i], h[i]);
+            Rw::unpack(ng[i], g[i]);
+            d[i] = nd[i];
+            if (P.R != nullptr) {
+                float r[V];
+                Rw::unpack(nr[i], r);
 #pragma unroll
-                    for (int j = 0; j < V; ++j) h[i][j] += r[j];
-                }
+                for (int j = 0; j < V; ++j) h[i][j] += r[j];
             }
+        }
+        if (r0 + stride < P.rows) ahead(row + stride);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float wv[V];
+            Rw::unpack(w[i], wv);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 h[i][j] *= rstd;                                  // xhat
                 dw[i][j] = fmaf(g[i][j], h[i][j], dw[i][j]);
-                g[i][j] *= w[i][j];
+                g[i][j] *= wv[j];
                 a = fmaf(g[i][j], h[i][j], a);
             }
         }
@@ -247,13 +269,13 @@ __global__ __launch_bounds__(RN_THREADS) void rmsnorm_bwd_kernel(const NormBwdAr
         for (int i = 0; i < NV; ++i) {
             const int c = (t + i * TPR) * V, n = live ? P.C - c : 0;
             if (n > 0) {
-                float d[V];
+                float o[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) d[j] = 0.f;
-                if (P.D != nullptr) Rw::load(P.D + (row * P.C + c) * E, n, d);
+                for (int j = 0; j < V; ++j) o[j] = 0.f;
+                if (P.D != nullptr) Rw::unpack(d[i], o);
 #pragma unroll
-                for (int j = 0; j < V; ++j) d[j] = fmaf(rstd, g[i][j] - h[i][j] * a, d[j]);
-                Rw::store(P.dX + (row * P.C + c) * E, n, d);
+                for (int j = 0; j < V; ++j) o[j] = fmaf(rstd, g[i][j] - h[i][j] * a, o[j]);
+                Rw::store(P.dX + (row * P.C + c) * E, n, o);
             }
         }
     }
@@ -374,8 +396,13 @@ static Shape row_shape(long nv, int least) {
     return {0, 0};
 }
 
-// workgroups of a forward launch (the kernels walk on from there: a grid may not hold more than 2^32 threads)
-static unsigned grid_of(long blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)); }
+// workgroups of a forward launch; the kernels walk on from there.  Rows of one wave or less: 8 per CU (16 with the 8-bit output)
+// stay and keep their weights' lines (98304 x 256 bf16: 35.4 us = 5.7 TB/s against 41.5 with one group of rows per workgroup; 8-bit
+// 34.1 against 36.7); whole-workgroup rows: one each (8192 x 4096: 49.4 against 56.2), up to what a grid may hold.
+static unsigned grid_of(long blocks, int tpr, int mode) {
+    const long most = tpr > 64 ? 1 << 20 : dsw_device_cus() * (mode == RN_NORM ? 8 : 16);
+    return (unsigned)(blocks < most ? blocks : most);
+}
 
 #define RN_SHAPES(CASE) CASE(16, 1) CASE(32, 1) CASE(64, 1) CASE(64, 2) CASE(64, 4) CASE(256, 2) CASE(256, 4) CASE(256, 8)
 
@@ -384,13 +411,13 @@ static int launch_fwd(const NormArgs& a, hipStream_t s) {
     constexpr int V = Row<BF16>::V;
     const Shape sh = row_shape((a.C + V - 1) / V, MODE == RN_NORM ? 16 : 128 / V);
     if (sh.tpr == 0) {
-        DSW_LAUNCH((rmsnorm_fwd_long_kernel<BF16, MODE>), dim3(grid_of(a.rows)), dim3(RN_THREADS), 0, s, a);
+        DSW_LAUNCH((rmsnorm_fwd_long_kernel<BF16, MODE>), dim3(grid_of(a.rows, RN_THREADS, MODE)), dim3(RN_THREADS), 0, s, a);
         return dsw_check_launch();
     }
     const long blocks = (a.rows + RN_THREADS / sh.tpr - 1) / (RN_THREADS / sh.tpr);
 #define CASE(T, N) \
     if (sh.tpr == T && sh.nv == N) { \
-        DSW_LAUNCH((rmsnorm_fwd_kernel<BF16, T, N, MODE>), dim3(grid_of(blocks)), dim3(RN_THREADS), 0, s, a); \
+        DSW_LAUNCH((rmsnorm_fwd_kernel<BF16, T, N, MODE>), dim3(grid_of(blocks, T, MODE)), dim3(RN_THREADS), 0, s, a); \
         return dsw_check_launch(); \
     }
     RN_SHAPES(CASE)
@@ -398,9 +425,9 @@ static int launch_fwd(const NormArgs& a, hipStream_t s) {
     return DSW_ERR_BAD_ARG;
 }
 
-// workgroups of the backward pass (= rows of `part`): enough to fill the card, few enough that the partial rows stay small
-// against the tensors
-constexpr int RN_BWD_BLOCKS = 1024;
+// workgroups of the backward pass (= rows of `part`): two per CU, each with the next row in flight (98304 x 256 bf16: 47.4 us =
+// 5.3 TB/s; 768: 48.6, 1024: 52.9; without the next row ahead 52.5 at 1024 and 78.7 at 512.  8192 x 4096: 69.4, 74.7, 79.8)
+constexpr int RN_BWD_BLOCKS = 512;
 static long bwd_blocks(int64_t rows, int64_t C, int dtype) {
     const int V = dtype == DSW_BF16 ? 8 : 4;
     const Shape sh = row_shape((C + V - 1) / V, 16);
@@ -415,7 +442,7 @@ static int launch_bwd(const NormBwdArgs& a, char* dW, hipStream_t s) {
     const Shape sh = row_shape((a.C + V - 1) / V, 16);
     const long blocks = bwd_blocks(a.rows, a.C, BF16 ? DSW_BF16 : DSW_F32);
     if (sh.tpr == 0) {
-        if (a.dX != nullptr && a.rows > 0) DSW_LAUNCH(rmsnorm_bwd_long_dx_kernel<BF16>, dim3(grid_of(a.rows)), dim3(RN_THREADS), 0, s, a);
+        if (a.dX != nullptr && a.rows > 0) DSW_LAUNCH(rmsnorm_bwd_long_dx_kernel<BF16>, dim3(grid_of(a.rows, RN_THREADS, RN_NORM)), dim3(RN_THREADS), 0, s, a);
         if (a.part != nullptr)
             DSW_LAUNCH(rmsnorm_bwd_long_dw_kernel<BF16>, dim3((unsigned)((a.C + RN_THREADS - 1) / RN_THREADS), (unsigned)blocks),
                        dim3(RN_THREADS), 0, s, a);

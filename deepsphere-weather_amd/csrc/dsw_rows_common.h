@@ -35,7 +35,7 @@ struct Row {
         u32x4 t;
         if constexpr (BF16) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) t[j] = f32_to_bf16(v[2 * j]) | ((uint32_t)f32_to_bf16(v[2 * j + 1]) << 16);
+            for (int j = 0; j < 4; ++j) t[j] = f32x2_to_bf16(v[2 * j], v[2 * j + 1]);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) t[j] = __float_as_uint(v[j]);
@@ -44,6 +44,10 @@ struct Row {
     }
     static __device__ __forceinline__ u32x4 raw(const char* p) { return reinterpret_cast<const Any*>(p)->v; }
     static __device__ __forceinline__ void put_raw(char* p, const u32x4 t) { reinterpret_cast<Any*>(p)->v = t; }
+    static __device__ __forceinline__ void put_raw_stream(char* p, const u32x4 t) {            // past the caches
+        typedef uint32_t __attribute__((ext_vector_type(4), aligned(1))) any4;
+        __builtin_nontemporal_store((any4)t, reinterpret_cast<any4*>(p));
+    }
     // channels [0, n) of the 16 bytes at p; the others come back as zero (n >= V: all of them)
     static __device__ __forceinline__ void load(const char* p, int n, float (&v)[V]) {
         if (n >= V) {
@@ -52,6 +56,21 @@ struct Row {
 #pragma unroll
             for (int j = 0; j < V; ++j) v[j] = j < n ? one(p + j * E) : 0.f;
         }
+    }
+    // the same without the conversion: a lane's 16 bytes with zeros behind channel n (n <= 0: nothing is read)
+    static __device__ __forceinline__ u32x4 fetch(const char* p, int n) {
+        u32x4 t = {0u, 0u, 0u, 0u};
+        if (n >= V) {
+            t = reinterpret_cast<const Any*>(p)->v;
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (j < n) {
+                    if constexpr (BF16) t[j / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(p + j * E) << (16 * (j & 1));
+                    else t[j] = *reinterpret_cast<const uint32_t*>(p + j * E);
+                }
+        }
+        return t;
     }
     static __device__ __forceinline__ void store(char* p, int n, const float (&v)[V]) {
         if (n >= V) {

@@ -459,6 +459,25 @@ def test_clip_leaves_what_lies_between_and_reads_every_layout():
     F.clip_grad_norm_([flat[:100], flat[50:200]], 1.0, out=[torch.empty(100, device=DEV), torch.empty(150, device=DEV)])   # reads may
 
 
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 36_000_003), (torch.bfloat16, 70_000_001)])
+def test_clip_of_more_than_the_caches_hold(dtype, n):
+    """The results leave past the caches: into another tensor and in place, at an odd address, with a second tensor behind."""
+    flat = torch.randn(n + 100, device=DEV).to(dtype)
+    g, small = flat[3:3 + n], flat[n + 50:n + 90]
+    keep = flat.clone()
+    out = torch.zeros_like(flat)
+    to = [out[3:3 + n], out[n + 50:n + 90]]
+    norm = F.clip_grad_norm_([g, small], 1.0, out=to)
+    want = math.sqrt(float(g.double().square().sum()) + float(small.double().square().sum()))
+    assert abs(float(norm) - want) <= 2 * U * want and torch.equal(flat, keep)
+    for a, b in zip((g, small), to):
+        w = a.double() / (want + 1e-6)
+        assert bool(((b.double() - w).abs() <= (HALF[dtype] + 3 * U) * w.abs()).all())
+    assert bool((out[:3] == 0).all()) and bool((out[3 + n:n + 50] == 0).all()) and bool((out[n + 90:] == 0).all())
+    assert torch.equal(F.clip_grad_norm_([g, small], 1.0), norm) and torch.equal(g, to[0]) and torch.equal(small, to[1])
+    assert torch.equal(flat[3 + n:n + 50], keep[3 + n:n + 50])
+
+
 def test_clip_of_neighbours_equals_one_flat_tensor():
     flat = torch.randn(100003, device=DEV)
     cuts = [0, 1, 30, 31, 5000, 77777, 100003]
