@@ -95,16 +95,13 @@ static __device__ __forceinline__ void store_out(void* p, long i, float v) {
 }
 
 // Global memory -> LDS without registers: lane l's 16 (4) bytes land at LDS byte `lds` + 16 l (4 l).  The compiler does not count
-// these loads: they are waited for by hand.
+// these loads: they are waited for by hand.  (m0 holds no value of the compiler's between instructions: it is a reserved register that
+// it sets right before an instruction of its own that reads it, of which there is none here.)
 static __device__ __forceinline__ void load_to_lds(const uint8_t* base, uint32_t off, uint32_t lds) {
-    uint32_t m0;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-                 : "=&s"(m0) : "v"(off), "s"(base), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(lds) : "memory");
 }
 static __device__ __forceinline__ void load_to_lds4(const float* at, uint32_t lds) {
-    uint32_t m0;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(m0) : "v"(at), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(at), "s"(lds) : "memory");
 }
 static __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 static __device__ __forceinline__ uint32_t lds_byte(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
@@ -203,8 +200,11 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
     constexpr int STAGE = ROWS * 8 + WAVES * 16;       // 16-byte units: the rows, then 64 row scales of each wave
     static_assert(ROWS % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "a wave's pieces lie in one operand each");
     static_assert(128 % (16 * NT) == 0, "a wave's outputs share a row of weight scales");
-    constexpr int GO = (PIECES + MT) / MT;             // loads issued with each of the last step's products
-    static_assert(MT <= 4 && NT >= 2 && NT % 2 == 0, "");
+    // A block's loads are issued one by one between products (a load costs its wave three scalar instructions; 9 of them behind one
+    // another left the matrix cores waiting): GO with each product of the last step of the block before the previous one, the
+    // rest from there on.
+    constexpr int GO = (PIECES + NT * MT - MT) / (NT * MT - MT), FIRST = MT * GO < PIECES ? MT * GO : PIECES;
+    static_assert(MT <= 4 && NT >= 2 && NT % 2 == 0 && FIRST + (NT - 1) * MT * GO > PIECES, "every load is issued before it is waited for");
     extern __shared__ u32x4 lds[];                     // [2][STAGE]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int tn, tm;
@@ -258,10 +258,8 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
         fetch_scales(0);
         advance(whole > 1);
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) fetch_piece(i, off[i], 1);
-        fetch_scales(1);
-        advance(whole > 2);
-        asm volatile("s_waitcnt vmcnt(%0)" :: "n"(PIECES + 1) : "memory");     // block 0 is there, block 1 on its way
+        for (int i = 0; i < FIRST; ++i) fetch_piece(i, off[i], 1);
+        asm volatile("s_waitcnt vmcnt(%0)" :: "n"(FIRST) : "memory");          // block 0 is there, block 1 on its way
         __syncthreads();
         Frag<WIDE> fx[MT], fw = make_frag<WIDE>(lds[w_lo], lds[w_hi]);
         float s[MT], s_old[MT];
@@ -299,9 +297,12 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
                     if (t + 1 == NT) {
                         fx[j] = make_frag<WIDE>(there[x_lo + 128 * j], there[x_hi + 128 * j]);
 #pragma unroll
-                        for (int i = j * GO; i < (j + 1) * GO; ++i) {          // block b + 2
-                            if (i < PIECES) fetch_piece(i, off[i], stage);
-                            else if (i == PIECES) fetch_scales(stage);
+                        for (int i = j * GO; i < (j + 1) * GO && i < FIRST; ++i) fetch_piece(i, off[i], stage);      // block b + 2
+                    } else {
+#pragma unroll
+                        for (int i = FIRST + (t * MT + j) * GO; i < FIRST + (t * MT + j + 1) * GO; ++i) {            // block b + 1, the rest
+                            if (i < PIECES) fetch_piece(i, off[i], stage ^ 1);
+                            else if (i == PIECES) fetch_scales(stage ^ 1);
                         }
                     }
 #pragma unroll
@@ -309,10 +310,10 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_mix_tile_kernel(const MixArg
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 fw = next;
+                if (t + 2 == NT) advance(b + 2 < whole);                       // block b + 1 is sent for
             }
 #pragma unroll
             for (int j = 0; j < MT; ++j) { s_old[j] = s[j]; s[j] = s_next[j]; }
-            advance(b + 3 < whole);
             stage ^= 1;
         }
         wait_loads();
