@@ -19,7 +19,7 @@ typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 struct __attribute__((packed, aligned(1))) Any16 { u32x4 v; };
 
-constexpr int64_t MIX_LD_MAX = (1 << 24) - 1;      // a tile's rows are reached by 32-bit offsets
+constexpr int64_t MIX_LD_MAX = (1 << 23) - 1;      // a tile's 256 rows are reached by offsets below 2^31
 
 struct MixArgs {
     const uint8_t* X; const float* XS; const uint8_t* W; const float* WS; const void* bias; void* Y;
@@ -118,13 +118,13 @@ static __device__ __forceinline__ float scalar_load(const float* p, int i) {
 template <int NT>
 static __device__ __forceinline__ int w_place(int row) { return (row & 3) | (((row / (4 * NT)) & 1) << 2); }
 
-// tiles of a grid: each of the 8 dies takes a contiguous run of them (blocks go round the dies), 8 row tiles deep, so that the
+// tiles of a grid: each of the 8 dies takes a contiguous run of them (blocks go round the dies), 4 row tiles deep, so that the
 // tiles that one L2 serves at a time share rows and weights
 static __device__ __forceinline__ bool tile_of(int tiles_n, int tiles_m, int& tn, int& tm) {
     const int T = tiles_n * tiles_m, per = (T + 7) >> 3;
     const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if (id >= T) return false;
-    const int deep = 8, band = id / (deep * tiles_n), in = id - band * deep * tiles_n;
+    const int deep = 4, band = id / (deep * tiles_n), in = id - band * deep * tiles_n;
     const int high = tiles_m - band * deep < deep ? tiles_m - band * deep : deep;
     tn = in / high;
     tm = band * deep + in % high;
@@ -605,18 +605,22 @@ static int64_t mix_ws_bytes(int64_t M, int64_t N, int64_t K, bool aligned) {
 
 // Which kernel (time in us, bf16 output, aligned rows; "LDS" = fp8_mix_few_lds_kernel<2, 1, 8>, tiles as outputs n x rows m):
 //   rows x K x N        registers  LDS   32x128  128x128  256x256
-//   8 x 4096 x 4096         6.0    6.7    18.3     22.7
-//   64 x 8192 x 1024       21.7    8.9    32.6     41.3
-//   500 x 2048 x 512        8.1    5.1     9.8     12.2     30.1
-//   1000 x 256 x 1000      11.8    8.2     4.4      5.7     12.8
-//   1000 x 4096 x 1000     47.9   26.5    19.7     24.2     52.1
-//   24576 x 256 x 256      63.4           10.8      9.0     14.6
-//   98304 x 128 x 256     219             28.1     19.5     26.6
-//   4096 x 1024 x 4096    273             44.4     27.8     26.4
-//   4096 x 4096 x 4096    737            136       80.4     65.4
-// so: 16 rows at most - registers; as long as the LDS kernel's workgroups come to four per CU - that; the larger tiles as soon as
-// there is one for every CU (the largest from six blocks of K on: below, its fuller epilogue costs more than it saves).
-// fp32 output (bf16 matrix instructions): 128 x 128 tiles of four waves instead of eight (4096^3: 134 against 149), no larger ones.
+//   8 x 4096 x 4096         6.0    6.5    17.8     22.4     41.5
+//   64 x 8192 x 1024       21.1    8.8    32.3     42.9     79.1
+//   500 x 2048 x 512        7.8    5.2     7.9     10.2     23.5
+//   1000 x 256 x 1000       8.4    8.2     3.8      4.4      8.6
+//   1000 x 4096 x 1000     40.2   27.4    19.5     24.2     43.3
+//   6000 x 512 x 512       25.0   22.2     7.2      6.1     10.9
+//   24576 x 256 x 256      34.5   37.7    10.4      7.8      8.3
+//   98304 x 128 x 256     117    137      25.4     16.6     17.6
+//   98304 x 256 x 64       35.5   38.8    10.8     11.2     17.6
+//   4096 x 512 x 4096     111     99.8    30.8     19.1     17.9
+//   4096 x 4096 x 4096    577    294     144       78.1     62.6
+// so: 16 rows at most - registers; as long as the LDS kernel's workgroups come to four per CU - that; 128 x 128 as soon as there is
+// such a tile for every other CU (and more than 64 outputs), 256 x 256 as soon as there is one for every CU (from four blocks of
+// K on: below, its fuller epilogue costs more than it saves).
+// fp32 output (bf16 matrix instructions): 128 x 128 by four waves instead of eight (4096^3: 139 against 154) from one for every CU
+// on (6000 x 512 x 512: 11.3 against 10.1 of the 32 x 128), no larger ones.
 template <bool BF16>
 static int launch_mix(const MixArgs& a, hipStream_t s) {
     const long cus = dsw_device_cus();
@@ -628,8 +632,8 @@ static int launch_mix(const MixArgs& a, hipStream_t s) {
     }
     if (tiles(16, 32) <= 4 * cus) return launch_few_lds<2, 1, 8, BF16>(a, s);
     if constexpr (BF16) {
-        if (a.KB >= 6 && tiles(256, 256) >= cus) return launch_tile<8, 4, 2, 4, BF16>(a, s);
-        if (a.N > 64 && tiles(128, 128) >= cus) return launch_tile<4, 2, 2, 4, BF16>(a, s);
+        if (a.KB >= 4 && tiles(256, 256) >= cus) return launch_tile<8, 4, 2, 4, BF16>(a, s);
+        if (a.N > 64 && tiles(128, 128) >= cus / 2) return launch_tile<4, 2, 2, 4, BF16>(a, s);
     } else {
         if (a.N > 64 && tiles(128, 128) >= cus) return launch_tile<4, 4, 2, 2, BF16>(a, s);
     }

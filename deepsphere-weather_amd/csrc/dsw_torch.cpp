@@ -151,16 +151,23 @@ void refuse_foreign_leaves(const Tensor& t) {
         auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
         if (leaf == nullptr) continue;
         const auto s = leaf->stream();
-        TORCH_CHECK(!s || *s == here, "dsw: a backward pass is being captured while an earlier graph over the same leaf (shape ",
+        if (!s || *s == here) continue;
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;                      // (a stream of the same capture may join it)
+        const hipError_t err = hipStreamIsCapturing(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *s).stream(), &status);
+        if (err != hipSuccess) (void)hipGetLastError();
+        TORCH_CHECK(err == hipSuccess && status == hipStreamCaptureStatusActive, "dsw: a backward pass is being captured while an earlier graph over the same leaf (shape ",
                     leaf->variable.sizes(), ") is alive on another stream; drop that graph (its outputs, its loss) before the capture");
     }
 }
 
 // gradients that do not differentiate again: an error for whoever tries (create_graph), nothing otherwise
-variable_list once(variable_list grads) {
+// (their error stands behind everything they were computed from, so that no path past it reads as a missing gradient)
+variable_list once(variable_list grads, const variable_list& from, const variable_list& dys) {
     if (!at::GradMode::is_enabled()) return grads;
     variable_list in;
     for (Tensor& g : grads) if (g.defined()) in.push_back(g.detach().requires_grad_());
+    for (const auto& list : {from, dys})
+        for (const Tensor& t : list) if (t.defined()) in.push_back(t);
     auto err = std::make_shared<torch::autograd::DelayedError>("dsw: the row norm differentiates once", (int64_t)in.size());
     in = (*err)(std::move(in));
     size_t k = 0;
@@ -207,7 +214,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
         const auto saved = ctx->get_saved_variables();
         const auto g = norm_backward(saved[0], Tensor(), saved[1], saved[2], grads[0], Tensor(), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
-        return once({g[0], g[1], Tensor()});
+        return once({g[0], g[1], Tensor()}, saved, grads);
     }
 };
 
@@ -226,7 +233,7 @@ struct RmsNormResidual : torch::autograd::Function<RmsNormResidual> {
         const bool need_x = ctx->needs_input_grad(0), need_r = ctx->needs_input_grad(1);
         const auto saved = ctx->get_saved_variables();
         const auto g = norm_backward(saved[0], saved[3], saved[1], saved[2], grads[0], grads[1], need_x || need_r, ctx->needs_input_grad(2));
-        return once({need_x ? g[0] : Tensor(), need_r ? g[0] : Tensor(), g[1], Tensor()});
+        return once({need_x ? g[0] : Tensor(), need_r ? g[0] : Tensor(), g[1], Tensor()}, saved, grads);
     }
 };
 
@@ -315,7 +322,7 @@ Tensor dense_mix_fp8(const Tensor& xq, const Tensor& xs, const Tensor& wq, const
     no_backward("dense_mix_fp8", {&xs, &ws, &bias});
     on_gpu(xq);
     const c10::DeviceGuard guard(xq.device());
-    constexpr int64_t far = 1 << 24;                   // rows further apart are copied (the tiles use 32-bit offsets)
+    constexpr int64_t far = 1 << 23;                   // rows further apart are copied (the tiles use 32-bit offsets)
     const Tensor w = (k > 1 && wq.stride(1) != 1) || wq.stride(0) < k || wq.stride(0) >= far ? wq.contiguous() : wq;
     Rows x = as_rows(xq);
     if (x.step >= far) x = as_rows(xq.contiguous());

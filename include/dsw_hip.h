@@ -441,7 +441,7 @@ int dsw_rmsnorm_bwd(const void* G, const void* D, const void* X, int64_t ldx, co
 
 /* Per-node linear map of e4m3 rows and e4m3 weights, a scale per block of 128:
  *     Y[m, n] = sum_b XS[m * xs_row + b * xs_blk] * WS[(n / 128) * ceil(K / 128) + b] * sum_{k in block b} X[m, k] W[n, k] + bias[n]
- * X: M rows of K bytes, ldx apart; W: N rows of K bytes, ldw apart (both < 2^24); bias [N] of dtype or NULL; Y [M][N] dense, dtype = its type.
+ * X: M rows of K bytes, ldx apart; W: N rows of K bytes, ldw apart (both < 2^23); bias [N] of dtype or NULL; Y [M][N] dense, dtype = its type.
  * Any K, N >= 1 and alignments; rows that are not 16-byte aligned or no multiple of 16 bytes long (aligned = 0; bases, strides and K
  * of both operands) are copied into the workspace first when there are more than 64 of them.  The order of every sum is fixed by the sizes.  fp32 output: exact products, fp32 sums.  bf16
  * output: the 8-bit matrix instructions, which within 8 neighbouring k drop what lies 13 bits below the largest product, then sum

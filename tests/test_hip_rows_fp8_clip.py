@@ -142,6 +142,53 @@ def test_norm_partial_gradients_and_layouts():
     assert torch.equal(torch.autograd.grad(y, xl, gt)[0], full[0])
 
 
+def test_norm_differentiates_once():
+    x, w = torch.randn(5, 32, device=DEV, requires_grad=True), torch.ones(32, device=DEV, requires_grad=True)
+    for y in (F.rms_norm(x, w), F.rms_norm_residual(x, x, w)[0]):
+        (g,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiates once"):
+            torch.autograd.grad(g.sum(), x)
+
+
+def test_norm_saves_what_it_reads():
+    """An input that changes before backward is noticed, whichever tensors backward reads again."""
+    for dtype in DTYPES:
+        x, r, w = (t.to(DEV) for t in _norm_inputs(4, 40, dtype, True))
+        w.requires_grad_()
+        y, h = F.rms_norm_residual(x, r, w)
+        (x if dtype == torch.bfloat16 else h).mul_(2)
+        with pytest.raises(RuntimeError, match="inplace|in-place"):
+            torch.autograd.grad(y.float().sum(), w)
+
+
+def test_beyond_32_bits():
+    """More than 2^31 elements and 2^32 bytes in every operand: first and last rows against calls on them alone."""
+    rows, C = 530_000, 4100
+    x = torch.empty(rows, C, dtype=torch.bfloat16, device=DEV)
+    ends = torch.randn(8, C, device=DEV).bfloat16()
+    x.fill_(0.5)
+    x[:4], x[-4:] = ends[:4], ends[4:]
+    w = torch.randn(C, device=DEV).bfloat16()
+    y = F.rms_norm(x, w)
+    alone = F.rms_norm(ends, w)
+    assert torch.equal(y[:4], alone[:4]) and torch.equal(y[-4:], alone[4:])
+    del y
+    q, q8 = F.quantize_fp8(x), F.quantize_fp8(ends)
+    assert torch.equal(q.q[-4:].view(torch.uint8), q8.q[4:].view(torch.uint8)) and torch.equal(q.scale[-4:], q8.scale[4:])
+    m8 = F.quantize_fp8_weight(torch.randn(C, 4200, device=DEV))
+    y = F.dense_mix_fp8(q, m8)                                   # 2.2 G outputs
+    tail = F.Fp8Rows(q.q[-600:], q.scale[-600:])
+    part = F.dense_mix_fp8(tail, m8)
+    assert y.shape == (rows, 4200) and float((y[-600:].float() - part.float()).abs().max()) <= 2.0 ** -7 * float(part.float().abs().max())
+    assert torch.equal(y[600:700], y[100_000:100_100])             # equal rows, equal bits, wherever they lie in a tile row of 16
+    del y, q
+    norm = F.clip_grad_norm_(x.view(-1), 1.0)
+    want = math.sqrt(float(ends.double().square().sum()) + 0.25 * (rows - 8) * C)
+    assert abs(float(norm) - want) <= 4 * U * want
+    room = (HALF[torch.bfloat16] + 3 * U) * float(ends.float().abs().max()) / want
+    assert float((x[-4:].double() - ends[4:].double() / (want + 1e-6)).abs().max()) <= room
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_norm_special_values_stay_in_their_rows(dtype):
     x, _, w = _norm_inputs(6, 300, dtype, False, 3)
@@ -323,6 +370,12 @@ def test_product_layouts(rows):
     same = F.dense_mix_fp8(F.Fp8Rows(xq.to(DEV), xs[:1].to(DEV).expand(rows, 3)), F.Fp8Weight(wq.to(DEV), ws.to(DEV)), dtype=torch.float32)
     want, mag = _mix64(xq, xs[:1].expand(rows, 3), wq, ws)
     _within(same, want, _mix_tol(want, mag, K, torch.float32), "one scale for all rows")
+    per_row = F.dense_mix_fp8(F.Fp8Rows(xq.to(DEV), xs[:, :1].to(DEV).expand(rows, 3)), F.Fp8Weight(wq.to(DEV), ws.to(DEV)), dtype=torch.float32)
+    want, mag = _mix64(xq, xs[:, :1].expand(rows, 3), wq, ws)
+    _within(per_row, want, _mix_tol(want, mag, K, torch.float32), "one scale for all blocks")
+    one = F.dense_mix_fp8(F.Fp8Rows(xq[0].to(DEV), xs[0].to(DEV)), F.Fp8Weight(wq.to(DEV), ws.to(DEV)), dtype=torch.float32)
+    want, mag = _mix64(xq[:1], xs[:1], wq, ws)
+    _within(one.view(1, N), want, _mix_tol(want, mag, K, torch.float32), "no leading axis")
     none = F.dense_mix_fp8(F.Fp8Rows(xq[:0].to(DEV), xs[:0].to(DEV)), F.Fp8Weight(wq.to(DEV), ws.to(DEV)))
     assert none.shape == (0, N)
 
