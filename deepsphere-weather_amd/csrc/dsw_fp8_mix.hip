@@ -652,7 +652,8 @@ static int align_rows(const MixArgs& a, uint8_t* out, hipStream_t s) {
 extern "C" {
 
 static bool mix_sizes_ok(int64_t M, int64_t N, int64_t K) {
-    return M >= 0 && N >= 1 && K >= 1 && M <= 0x7fffffff - 256 && N <= (1 << 22) && K <= MIX_LD_MAX - 15;
+    return M >= 0 && N >= 1 && K >= 1 && M <= 0x7fffffff - 256 && N <= (1 << 22) && K <= MIX_LD_MAX - 15 &&
+           (M + 127) / 128 * ((N + 31) / 32) < (1 << 24) - 8;          // (a grid has less than 2^32 threads)
 }
 
 int64_t dsw_fp8_mix_workspace_bytes(int64_t M, int64_t N, int64_t K, int aligned) {

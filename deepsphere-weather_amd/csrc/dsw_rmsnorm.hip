@@ -6,8 +6,8 @@
 // All of it is bound by HBM: a row is read once into registers (16 bytes per lane and access), the sums run over the lanes that
 // share the row, and everything that a pass can derive from the row leaves in the same pass.  The square sum and the norm use
 // the unrounded fp32 sum x + r; h itself is rounded to the storage type once.  The backward pass takes the two addends rather than
-// the rounded h: with bf16 storage the rounding would be as large an error in dw as dw's own (1.5 x together; a fifth stream
-// read, 10 us of 84 at 98304 x 256).
+// the rounded h: with bf16 storage the rounding would be as large an error in dw as dw's own (1.5 x together); the price is
+// a fifth stream, 50 MB of 250 at 98304 x 256.
 #include "dsw_rows_common.h"
 #include "../../include/dsw_hip.h"
 

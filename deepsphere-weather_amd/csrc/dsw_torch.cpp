@@ -3,7 +3,8 @@
 // The kernels are the C entries of libdsw_hip.so (include/dsw_hip.h); this file checks arguments, allocates results on the current
 // stream and records backward passes.  It is compiled code because of what the operators are used for: one token is normalised
 // in 4 us and multiplied in 5 us on the card, and a training step's norm spends less time there than an interpreter needs to
-// run its forward and backward functions on two threads (measured: a Python autograd function 150 us, this one 45-60 us).
+// run its forward and backward functions on two threads (777 x 1030 fp32, both passes: a Python autograd function 150 us, this
+// one 54 us).
 //
 // Errors: ValueError / TypeError for arguments, RuntimeError for what the path does not offer and for the library's codes.
 #include <torch/extension.h>
@@ -147,9 +148,9 @@ void refuse_foreign_leaves(const Tensor& t) {
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
     const c10::Stream here = c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device());
-    for (const auto& edge : node->next_edges()) {
-        auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
-        if (leaf == nullptr) continue;
+    for (size_t i = 0; i < node->num_outputs(); ++i) {
+        auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(node->next_edge(i).function.get());
+        if (leaf == nullptr || !node->task_should_compute_output(i)) continue;
         const auto s = leaf->stream();
         if (!s || *s == here) continue;
         hipStreamCaptureStatus status = hipStreamCaptureStatusNone;                      // (a stream of the same capture may join it)

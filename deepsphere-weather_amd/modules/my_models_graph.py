@@ -103,7 +103,7 @@ class _NodeLinear(Linear):
     def serve_fp8(self, enable=True):
         """Inference through the 8-bit channel mix: the weight is quantised now (a scale per 128 x 128 block), the input rows
         in each call.  Only calls under ``torch.no_grad()`` take it; moving or casting the module switches it off, and a weight
-        that has changed since raises (call it again)."""
+        that has changed since raises (call it again; writes through ``weight.data`` are not noticed)."""
         with torch.no_grad():
             self._fp8 = (dsw_functional.quantize_fp8_weight(self.weight.t()), self.weight._version) if enable else None
         return self

@@ -150,6 +150,21 @@ def test_norm_differentiates_once():
             torch.autograd.grad(g.sum(), x)
 
 
+def test_addends_do_not_share_a_gradient():
+    x, r, w = (t.to(DEV).requires_grad_() for t in _norm_inputs(6, 64, torch.float32, True))
+    y, h = F.rms_norm_residual(x, r, w)
+    (y.sum() + h.sum()).backward()
+    assert torch.equal(x.grad, r.grad) and x.grad.data_ptr() != r.grad.data_ptr()
+    F.clip_grad_norm_([x.grad, r.grad, w.grad], 0.5)
+    x2 = x.detach().clone().requires_grad_()
+    y, h = F.rms_norm_residual(x2, x2, w.detach())                   # the same tensor twice: both shares arrive
+    (y.sum() + h.sum()).backward()
+    xs = (x.detach() * 2).requires_grad_()
+    (F.rms_norm(xs, w.detach()).sum() + xs.sum()).backward()
+    # (the sum D + rstd (...) is rounded once in one pass, and once more when the two gradients are added by autograd)
+    assert float((x2.grad - 2 * xs.grad).abs().max()) <= 2 * 4 * U * (1 + float(xs.grad.abs().max()))
+
+
 def test_norm_saves_what_it_reads():
     """An input that changes before backward is noticed, whichever tensors backward reads again."""
     for dtype in DTYPES:

@@ -137,6 +137,8 @@ def test_c_entries_refuse_before_they_launch():
     assert lib.dsw_fp8_mix_workspace_bytes(1000, 8, 20, 1) == 0 and lib.dsw_fp8_mix_workspace_bytes(1000, 8, 20, 0) == 1008 * 32
     assert lib.dsw_fp8_mix(p, 20, p, 1, 1, p, 20, p, None, p, 1000, 8, 20, 0, p, 100, None) == -3
     assert lib.dsw_fp8_mix(p, 8, p, 1, 1, p, 7, p, None, p, 4, 8, 8, 0, None, 0, None) == -1
+    assert lib.dsw_fp8_mix(p, 8, p, 1, 1, p, 8, p, None, p, 1 << 30, 1 << 8, 8, 0, p, 1 << 50, None) == -1      # 2^26 tiles
+    assert lib.dsw_fp8_mix(p, 1 << 23, p, 1, 1, p, 8, p, None, p, 4, 8, 8, 0, None, 0, None) == -1
     assert lib.dsw_fp8_mix(p, 8, p, 1, 1, p, 8, p, None, p, 4, 8, 8, 5, None, 0, None) == -2
     assert lib.dsw_fp8_mix(None, 8, None, 1, 1, None, 8, None, None, None, 0, 8, 8, 0, None, 0, None) == 0
     assert b"overlap" in lib.dsw_strerror(-6)
