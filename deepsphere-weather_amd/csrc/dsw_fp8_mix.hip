@@ -468,16 +468,19 @@ __global__ __launch_bounds__(64 * WV) void fp8_mix_few_kernel(const MixArgs P) {
     }
 }
 
-// The same split for 16-byte aligned rows of whole 16-byte chunks and more than 16 rows m: a lane's share of a fragment lies in 16
+// The same split for 16-byte aligned rows of whole 16-byte chunks: a lane's share of a fragment lies in 16
 // rows' lines, so reading it straight into registers asks for 64 lines a load (measured: 15 bytes a clock and CU, and the rows m
 // are read again by every workgroup); here each wave has its block's rows brought into its own part of LDS, 8 whole lines a
 // load, reads its fragments there and sends for its next block before it multiplies.  No wave waits for another until the sums
 // are joined.
-template <int MT, int NT, int WV, bool BF16>
+//
+// S = 2: two blocks of a wave under way, with larger tiles in as much LDS: half the round trips, fewer copies of the rows m.
+template <int MT, int NT, int WV, int S, bool BF16>
 __global__ __launch_bounds__(64 * WV) void fp8_mix_few_lds_kernel(const MixArgs P) {
     constexpr bool WIDE = !BF16;
-    constexpr int ROWS = 16 * (NT + MT);
-    extern __shared__ u32x4 lds[];                     // [WV][ROWS][8], then [WV][NT MT 4][64] sums in the same place
+    constexpr int ROWS = 16 * (NT + MT), LOADS = ROWS / 8;
+    constexpr int U = 4;                               // blocks of a wave whose scales are loaded together (S = 2)
+    extern __shared__ u32x4 lds[];                     // [WV][S][ROWS][8], then [WV][NT MT 4][64] sums in the same place
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
     const int r16 = lane & 15, g = lane >> 4;
@@ -495,29 +498,24 @@ __global__ __launch_bounds__(64 * WV) void fp8_mix_few_lds_kernel(const MixArgs 
 #pragma unroll
     for (int j = 0; j < MT; ++j) xs[j] = P.XS + (long)(m0 + 16 * j + r16 < P.M ? m0 + 16 * j + r16 : P.M - 1) * P.xs_row;
     const float* const ws = P.WS + (long)(n0 >> 7) * P.KB;
-    u32x4* const own = lds + wave * ROWS * 8;
-    const uint32_t to = lds_byte(lds) + (uint32_t)(wave * ROWS * 128);
+    const uint32_t to = lds_byte(lds) + (uint32_t)(wave * S * ROWS * 128);
     const int whole = P.K >> 7, tail = P.K & 127;
-    auto fetch = [&](int b) {
+    auto fetch = [&](int b, int stage) {
 #pragma unroll
-        for (int i = 0; i < ROWS / 8; ++i)
-            load_to_lds((i < 2 * NT ? wbase : xbase) + (long)b * 128, b < whole || c16 < tail ? off[i] : off[i] - c16, to + 1024 * i);
+        for (int i = 0; i < LOADS; ++i)
+            load_to_lds((i < 2 * NT ? wbase : xbase) + (long)b * 128, b < whole || c16 < tail ? off[i] : off[i] - c16, to + (stage * ROWS * 8 + 64 * i) * 16);
     };
     f32x4 acc[NT][MT];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int j = 0; j < MT; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (wave < P.KB) fetch(wave);
-    for (int b = wave; b < P.KB; b += WV) {
-        float s[MT];
-        const float sw = scalar_load(ws, b);
-#pragma unroll
-        for (int j = 0; j < MT; ++j) s[j] = xs[j][(long)b * P.xs_blk];
-        wait_loads();
+    // block b out of its stage, whose place then takes block `next`
+    auto add = [&](int b, int stage, int next, const float (&s)[MT]) {
+        u32x4* const own = lds + (wave * S + stage) * ROWS * 8;
         if (b == whole && c16 >= tail) {               // the short last block: clear what lies behind the rows
 #pragma unroll
-            for (int i = 0; i < ROWS / 8; ++i) own[64 * i + lane] = u32x4{0u, 0u, 0u, 0u};
+            for (int i = 0; i < LOADS; ++i) own[64 * i + lane] = u32x4{0u, 0u, 0u, 0u};
         }
         const int lo = r16 * 8 + (g ^ (r16 & 7)), hi = r16 * 8 + ((g + 4) ^ (r16 & 7));
         u32x4 wc[NT][2], xc[MT][2];
@@ -527,19 +525,54 @@ __global__ __launch_bounds__(64 * WV) void fp8_mix_few_lds_kernel(const MixArgs 
         for (int j = 0; j < MT; ++j) { xc[j][0] = own[128 * (NT + j) + lo]; xc[j][1] = own[128 * (NT + j) + hi]; }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the fragments are in registers: their place may be filled again
         __builtin_amdgcn_sched_barrier(0);
-        if (b + WV < P.KB) fetch(b + WV);
+        if (next < P.KB) fetch(next, stage);
         Frag<WIDE> fw[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) fw[t] = make_frag<WIDE>(wc[t][0], wc[t][1]);
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
             const Frag<WIDE> fx = make_frag<WIDE>(xc[j][0], xc[j][1]);
-            const float sj = sw * s[j];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const f32x4 p = block_product<WIDE>(fw[t], fx);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) acc[t][j][q] = fmaf(p[q], sj, acc[t][j][q]);
+                for (int q = 0; q < 4; ++q) acc[t][j][q] = fmaf(p[q], s[j], acc[t][j][q]);
+            }
+        }
+    };
+    if constexpr (S == 1) {
+        if (wave < P.KB) fetch(wave, 0);
+        for (int b = wave; b < P.KB; b += WV) {
+            float s[MT];
+            const float sw = scalar_load(ws, b);
+#pragma unroll
+            for (int j = 0; j < MT; ++j) s[j] = xs[j][(long)b * P.xs_blk] * sw;
+            wait_loads();
+            add(b, 0, b + WV, s);
+        }
+    } else {
+        // The scales of U blocks are loaded in front of everything else: a load that the compiler knows of is waited for with all
+        // that was sent for behind it.
+        for (int b0 = wave; b0 < P.KB; b0 += U * WV) {
+            float s[U][MT];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int b = b0 + u * WV < P.KB ? b0 + u * WV : P.KB - 1;
+                const float sw = scalar_load(ws, b);
+#pragma unroll
+                for (int j = 0; j < MT; ++j) s[u][j] = xs[j][(long)b * P.xs_blk] * sw;
+            }
+            if (b0 == wave) {
+                fetch(b0, 0);
+                if (b0 + WV < P.KB) fetch(b0 + WV, 1);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int b = b0 + u * WV;
+                if (b >= P.KB) break;                  // (uniform)
+                if (b + WV < P.KB) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(LOADS) : "memory");
+                else wait_loads();
+                add(b, u & 1, b + 2 * WV, s[u]);
             }
         }
     }
@@ -584,10 +617,11 @@ static int launch_few(const MixArgs& a, hipStream_t s) {
                dim3(64 * WV), 0, s, a);
     return dsw_check_launch();
 }
-template <int MT, int NT, int WV, bool BF16>
+template <int MT, int NT, int WV, int S, bool BF16>
 static int launch_few_lds(const MixArgs& a, hipStream_t s) {
-    constexpr int stage = WV * 16 * (NT + MT) * 128, sums = WV * NT * MT * 1024, lds = stage > sums ? stage : sums;
-    auto* kernel = fp8_mix_few_lds_kernel<MT, NT, WV, BF16>;
+    constexpr int stage = WV * S * 16 * (NT + MT) * 128, sums = WV * NT * MT * 1024, lds = stage > sums ? stage : sums;
+    static_assert(lds <= 160 * 1024, "");
+    auto* kernel = fp8_mix_few_lds_kernel<MT, NT, WV, S, BF16>;
     if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
         return DSW_ERR_LAUNCH;
     DSW_LAUNCH(kernel, dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT))), dim3(64 * WV), lds, s, a);
@@ -603,34 +637,59 @@ static int64_t mix_ws_bytes(int64_t M, int64_t N, int64_t K, bool aligned) {
     return aligned || M <= MIX_FEW_ROWS ? 0 : (M + N) * ((K + 15) / 16 * 16);
 }
 
-// Which kernel (time in us, bf16 output, aligned rows; "LDS" = fp8_mix_few_lds_kernel<2, 1, 8>, tiles as outputs n x rows m):
-//   rows x K x N        registers  LDS   32x128  128x128  256x256
-//   8 x 4096 x 4096         6.0    6.5    17.8     22.4     41.5
-//   64 x 8192 x 1024       21.1    8.8    32.3     42.9     79.1
-//   500 x 2048 x 512        7.8    5.2     7.9     10.2     23.5
-//   1000 x 256 x 1000       8.4    8.2     3.8      4.4      8.6
-//   1000 x 4096 x 1000     40.2   27.4    19.5     24.2     43.3
-//   6000 x 512 x 512       25.0   22.2     7.2      6.1     10.9
-//   24576 x 256 x 256      34.5   37.7    10.4      7.8      8.3
-//   98304 x 128 x 256     117    137      25.4     16.6     17.6
-//   98304 x 256 x 64       35.5   38.8    10.8     11.2     17.6
-//   4096 x 512 x 4096     111     99.8    30.8     19.1     17.9
-//   4096 x 4096 x 4096    577    294     144       78.1     62.6
-// so: 16 rows at most - registers; as long as the LDS kernel's workgroups come to four per CU - that; 128 x 128 as soon as there is
-// such a tile for every other CU (and more than 64 outputs), 256 x 256 as soon as there is one for every CU (from four blocks of
-// K on: below, its fuller epilogue costs more than it saves).
+// Which kernel, aligned rows (times in us, bf16 output).  Few rows or outputs: the LDS kernel, named by its row tiles m, output tiles n
+// and blocks of a wave under way:
+//   rows x K x N        registers  1,1,1  1,1,2  2,1,1  2,1,2  3,1,1  4,1,2  4,2,1
+//   1 x 4096 x 4096         5.3     5.7    5.0
+//   16 x 8192 x 1024       10.1     7.5    6.1
+//   16 x 8192 x 8192       17.6    12.7   13.6
+//   17 x 4096 x 4096                6.7           6.8    5.8    7.3    6.7    9.1
+//   64 x 2048 x 1024                              3.6    3.7    4.2    4.9    7.9
+//   64 x 4096 x 2048                6.3           6.5    5.5    6.9    7.0   10.9
+//   48 x 8192 x 8192                             23.6   30.2   17.8   20.5   20.7
+//   128 x 4096 x 2048               9.0           8.4    9.4    8.8    7.4   11.2
+//   128 x 4096 x 4096              16.5          15.1   18.7   15.5   14.7   12.2
+//   90 x 2304 x 4096                8.2           7.1           7.0           9.1
+// so, with at least three blocks of K for a wave: two blocks under way and as few row tiles as leave no CU a second workgroup (they
+// would not fit next to each other); else all rows in one tile up to 64 of them.  With fewer blocks small workgroups of one
+// block under way, four to a CU.
+//
+// Then tiles by outputs n x rows m ("LDS": 2,1,1):
+//   rows x K x N          LDS   32x128  128x128  256x256
+//   64 x 8192 x 1024       8.8    32.3     42.9     79.1
+//   500 x 2048 x 512       5.2     7.9     10.2     23.5
+//   1000 x 256 x 1000      8.2     3.8      4.4      8.6
+//   1000 x 4096 x 1000    27.4    19.5     24.2     43.3
+//   6000 x 512 x 512      22.2     7.2      6.1     10.9
+//   24576 x 256 x 256     37.7    10.4      7.8      8.3
+//   98304 x 128 x 256    137      25.4     16.6     17.6
+//   98304 x 256 x 64      38.8    10.8     11.2     17.6
+//   4096 x 512 x 4096     99.8    30.8     19.1     17.9
+//   4096 x 4096 x 4096   294     144       78.1     62.6
+// as long as the LDS kernel's workgroups come to four per CU - that; 128 x 128 as soon as there is such a tile for every other CU
+// (and more than 64 outputs), 256 x 256 as soon as there is one for every CU (from four blocks of K on: below, its fuller
+// epilogue costs more than it saves).
 // fp32 output (bf16 matrix instructions): 128 x 128 by four waves instead of eight (4096^3: 139 against 154) from one for every CU
 // on (6000 x 512 x 512: 11.3 against 10.1 of the 32 x 128), no larger ones.
 template <bool BF16>
 static int launch_mix(const MixArgs& a, hipStream_t s) {
     const long cus = dsw_device_cus();
     auto tiles = [&](long n, long m) { return (a.N + n - 1) / n * ((a.M + m - 1) / m); };
-    if (a.M <= 16) return launch_few<1, 1, 4, 8, BF16>(a, s);
     if (!rows_aligned(a)) {                            // (at most MIX_FEW_ROWS: the caller has aligned the others)
+        if (a.M <= 16) return launch_few<1, 1, 4, 8, BF16>(a, s);
         if (a.M <= 32) return launch_few<2, 1, 1, 8, BF16>(a, s);
         return launch_few<4, 1, 1, 8, BF16>(a, s);
     }
-    if (tiles(16, 32) <= 4 * cus) return launch_few_lds<2, 1, 8, BF16>(a, s);
+    if (a.M <= 16) return a.KB > 8 && 2 * tiles(16, 16) <= 3 * cus ? launch_few_lds<1, 1, 8, 2, BF16>(a, s) : launch_few_lds<1, 1, 8, 1, BF16>(a, s);
+    if (a.KB > 16) {
+        if (tiles(16, 32) <= cus) return launch_few_lds<2, 1, 8, 2, BF16>(a, s);
+        if (tiles(16, 48) <= cus) return launch_few_lds<3, 1, 8, 2, BF16>(a, s);
+        if (tiles(16, 64) <= cus) return launch_few_lds<4, 1, 8, 2, BF16>(a, s);
+        if (a.M > 32 && a.M <= 48 && tiles(16, 48) <= 2 * cus) return launch_few_lds<3, 1, 8, 1, BF16>(a, s);
+        if (a.M > 48 && a.M <= 64 && tiles(16, 64) <= 2 * cus) return launch_few_lds<4, 1, 8, 1, BF16>(a, s);
+        if (a.M > 64 && a.KB >= 32 && tiles(32, 64) <= cus) return launch_few_lds<4, 2, 8, 1, BF16>(a, s);
+    }
+    if (tiles(16, 32) <= 4 * cus) return launch_few_lds<2, 1, 8, 1, BF16>(a, s);
     if constexpr (BF16) {
         if (a.KB >= 4 && tiles(256, 256) >= cus) return launch_tile<8, 4, 2, 4, BF16>(a, s);
         if (a.N > 64 && tiles(128, 128) >= cus / 2) return launch_tile<4, 2, 2, 4, BF16>(a, s);
