@@ -15,13 +15,14 @@ namespace {
 constexpr int GN_THREADS = 256;
 constexpr int GN_TENSORS = 144;            // segments per launch: their table travels as a kernel argument (< 4 KB), so a captured
                                            // graph owns its copy and no host buffer has to outlive the call
-constexpr int GN_AHEAD = 4;                // 16-byte loads of a thread in flight
-constexpr int GN_CHUNK = 256 * 32;         // elements of a workgroup's step: 4 (bf16) or 8 (fp32) loads of each thread
+// elements of a workgroup's step: 4 (bf16) or 8 (fp32) loads of each thread, all in flight (half as many: 9.5 us, 289; a quarter: 10.1,
+// 335, against 9.4 and 275 of 7 MB and 500 MB)
+constexpr int GN_CHUNK = 256 * 32;
 constexpr int GN_BLOCKS = 1024;            // partial sums of one launch at most
 constexpr int GN_MAX_PARTS = 16 * 1024;    // partial sums of one call at most
 
 // from here on the results leave past the caches, which keep what the first pass read last for the second, going backwards
-// (200 M gradients, 500 MB: 281 us against 314; 7 MB: no difference)
+// (200 M gradients, 500 MB: 277 us against 314; 7 MB: no difference)
 constexpr int64_t GN_STREAM_BYTES = (int64_t)128 << 20;
 
 struct GradTable {
@@ -65,19 +66,20 @@ static __device__ __forceinline__ double block_join(double s, double* red) {
 template <int P, bool BF16>
 static __device__ __forceinline__ double chunk_sum(const char* g, int n, double s) {
     using Rw = Row<BF16>;
-    constexpr int V = Rw::V;
+    constexpr int V = Rw::V, LOADS = GN_CHUNK / (GN_THREADS * V);
     int i = threadIdx.x * V;
-    for (; i + (GN_AHEAD - 1) * GN_THREADS * V + V <= n; i += GN_AHEAD * GN_THREADS * V) {
-        typename Rw::u32x4 t[GN_AHEAD];
+    if (n == GN_CHUNK) {
+        typename Rw::u32x4 t[LOADS];
 #pragma unroll
-        for (int q = 0; q < GN_AHEAD; ++q) t[q] = Rw::raw(g + (long)(i + q * GN_THREADS * V) * Rw::E);
+        for (int q = 0; q < LOADS; ++q) t[q] = Rw::raw(g + (long)(i + q * GN_THREADS * V) * Rw::E);
 #pragma unroll
-        for (int q = 0; q < GN_AHEAD; ++q) {
+        for (int q = 0; q < LOADS; ++q) {
             float v[V];
             Rw::unpack(t[q], v);
 #pragma unroll
             for (int j = 0; j < V; ++j) s = fold<P>(s, v[j]);
         }
+        return s;
     }
     for (; i < n; i += GN_THREADS * V) {
         float v[V];
@@ -111,26 +113,34 @@ static __device__ __forceinline__ double total_norm(const double* part, int npar
     return P == GN_L2 ? sqrt(s) : s;
 }
 
+// a whole chunk's loads of this thread, sent for in front of the norm that scales them
+template <bool BF16> struct Chunk { typename Row<BF16>::u32x4 t[GN_CHUNK / (GN_THREADS * Row<BF16>::V)]; };
+template <bool BF16>
+static __device__ __forceinline__ void chunk_load(const char* g, Chunk<BF16>& k) {
+    using Rw = Row<BF16>;
+#pragma unroll
+    for (int q = 0; q < GN_CHUNK / (GN_THREADS * Rw::V); ++q) k.t[q] = Rw::raw(g + (long)((threadIdx.x + q * GN_THREADS) * Rw::V) * Rw::E);
+}
 template <bool BF16, bool STREAM>
-static __device__ __forceinline__ void chunk_scale(const char* g, char* o, int n, float c) {
+static __device__ __forceinline__ void chunk_store(char* o, const Chunk<BF16>& k, float c) {
     using Rw = Row<BF16>;
     constexpr int V = Rw::V;
-    int i = threadIdx.x * V;
-    for (; i + (GN_AHEAD - 1) * GN_THREADS * V + V <= n; i += GN_AHEAD * GN_THREADS * V) {
-        typename Rw::u32x4 t[GN_AHEAD];
 #pragma unroll
-        for (int q = 0; q < GN_AHEAD; ++q) t[q] = Rw::raw(g + (long)(i + q * GN_THREADS * V) * Rw::E);
+    for (int q = 0; q < GN_CHUNK / (GN_THREADS * V); ++q) {
+        float v[V];
+        Rw::unpack(k.t[q], v);
 #pragma unroll
-        for (int q = 0; q < GN_AHEAD; ++q) {
-            float v[V];
-            Rw::unpack(t[q], v);
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[j] *= c;
-            if constexpr (STREAM) Rw::put_raw_stream(o + (long)(i + q * GN_THREADS * V) * Rw::E, Rw::pack(v));
-            else Rw::put_raw(o + (long)(i + q * GN_THREADS * V) * Rw::E, Rw::pack(v));
-        }
+        for (int j = 0; j < V; ++j) v[j] *= c;
+        char* const to = o + (long)((threadIdx.x + q * GN_THREADS) * V) * Rw::E;
+        if constexpr (STREAM) Rw::put_raw_stream(to, Rw::pack(v));
+        else Rw::put_raw(to, Rw::pack(v));
     }
-    for (; i < n; i += GN_THREADS * V) {
+}
+template <bool BF16>
+static __device__ __forceinline__ void part_scale(const char* g, char* o, int n, float c) {
+    using Rw = Row<BF16>;
+    constexpr int V = Rw::V;
+    for (int i = threadIdx.x * V; i < n; i += GN_THREADS * V) {
         float v[V];
         Rw::load(g + (long)i * Rw::E, n - i, v);
 #pragma unroll
@@ -144,20 +154,34 @@ template <int P, bool STREAM>
 __global__ __launch_bounds__(GN_THREADS) void grad_clip_kernel(const GradTable T, const double* part, int nparts, double max_norm,
                                                                float* norm) {
     __shared__ double red[4];
-    const double N = total_norm<P>(part, nparts, red);
-    if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)N;
-    if (T.n == 0) return;
-    const double q = max_norm / (N + 1e-6);
-    const float c = q > 1.0 ? 1.f : (float)q;                  // (a NaN stays one, as in max_norm / norm clamped from above)
-    for (long at_ = blockIdx.x; at_ < T.first[T.n]; at_ += gridDim.x) {
+    struct Place { const char* g; char* o; int n; bool bf16, in_place; };
+    auto place = [&](long at_) {
         const long chunk = T.first[T.n] - 1 - at_;             // from the end: what the first pass read last is still in the caches
         const int t = segment_of(T, chunk);
-        if (c == 1.f && T.g[t] == T.o[t]) continue;            // in place and nothing to clip: g * 1 is g
-        const long at = (chunk - T.first[t]) * GN_CHUNK;
-        const int n = chunk + 1 == T.first[t + 1] ? T.tail[t] + 1 : GN_CHUNK;
         const bool bf16 = T.bf16[t >> 5] >> (t & 31) & 1u;
-        if (bf16) chunk_scale<true, STREAM>(T.g[t] + at * 2, T.o[t] + at * 2, n, c);
-        else chunk_scale<false, STREAM>(T.g[t] + at * 4, T.o[t] + at * 4, n, c);
+        const long at = (chunk - T.first[t]) * GN_CHUNK * (bf16 ? 2 : 4);
+        return Place{T.g[t] + at, T.o[t] + at, chunk + 1 == T.first[t + 1] ? T.tail[t] + 1 : GN_CHUNK, bf16, T.g[t] == T.o[t]};
+    };
+    Chunk<true> half;
+    Chunk<false> full;
+    // (the first chunk travels while the partials are joined: 7 MB, both launches of a replayed graph 9.7 -> 9.4 us)
+    const bool work = T.n > 0 && blockIdx.x < T.first[T.n];
+    Place p = work ? place(blockIdx.x) : Place{};
+    if (work && p.n == GN_CHUNK) { if (p.bf16) chunk_load<true>(p.g, half); else chunk_load<false>(p.g, full); }
+    const double N = total_norm<P>(part, nparts, red);
+    if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)N;
+    if (!work) return;
+    const double q = max_norm / (N + 1e-6);
+    const float c = q > 1.0 ? 1.f : (float)q;                  // (a NaN stays one, as in max_norm / norm clamped from above)
+    for (long at_ = blockIdx.x;;) {
+        if (c == 1.f && p.in_place) {}                         // in place and nothing to clip: g * 1 is g
+        else if (p.n < GN_CHUNK) { if (p.bf16) part_scale<true>(p.g, p.o, p.n, c); else part_scale<false>(p.g, p.o, p.n, c); }
+        else if (p.bf16) chunk_store<true, STREAM>(p.o, half, c);
+        else chunk_store<false, STREAM>(p.o, full, c);
+        at_ += gridDim.x;
+        if (at_ >= T.first[T.n]) return;
+        p = place(at_);
+        if (p.n == GN_CHUNK && !(c == 1.f && p.in_place)) { if (p.bf16) chunk_load<true>(p.g, half); else chunk_load<false>(p.g, full); }
     }
 }
 
