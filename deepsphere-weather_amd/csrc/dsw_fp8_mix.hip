@@ -668,7 +668,13 @@ static int64_t mix_ws_bytes(int64_t M, int64_t N, int64_t K, bool aligned) {
 //   4096 x 4096 x 4096   294     144       78.1     62.6
 // as long as the LDS kernel's workgroups come to four per CU - that; 128 x 128 as soon as there is such a tile for every other CU
 // (and more than 64 outputs), 256 x 256 as soon as there is one for every CU (from four blocks of K on: below, its fuller
-// epilogue costs more than it saves).
+// epilogue costs more than it saves) and they cover at most a quarter more than 128 x 128 does.  Between them 128 x 64, three to a CU,
+// where they are at most one for every CU, or two over a single column of tiles (rows are read once either way):
+//   rows x K x N         128 x 64   else             rows x K x N         128 x 64   128 x 128   256 x 256
+//   8192 x 512 x 256        4.9      5.5             24576 x 512 x 128       7.0       7.6
+//   5000 x 1024 x 384       7.5      9.3             98304 x 512 x 128      19.4      17.8         25.0
+//   4096 x 4096 x 512      21.0     24.6             49152 x 1024 x 300     34.4      30.7         36.0
+//   6000 x 512 x 512        6.6      6.0             20000 x 4096 x 640     87.3      73.5         74.5
 // fp32 output (bf16 matrix instructions): 128 x 128 by four waves instead of eight (4096^3: 139 against 154) from one for every CU
 // on (6000 x 512 x 512: 11.3 against 10.1 of the 32 x 128), no larger ones.
 template <bool BF16>
@@ -691,7 +697,10 @@ static int launch_mix(const MixArgs& a, hipStream_t s) {
     }
     if (tiles(16, 32) <= 4 * cus) return launch_few_lds<2, 1, 8, 1, BF16>(a, s);
     if constexpr (BF16) {
-        if (a.KB >= 4 && tiles(256, 256) >= cus) return launch_tile<8, 4, 2, 4, BF16>(a, s);
+        if (a.KB >= 4 && tiles(256, 256) >= cus && 16 * tiles(256, 256) <= 5 * tiles(128, 128)) return launch_tile<8, 4, 2, 4, BF16>(a, s);
+        const long low = tiles(128, 64);
+        if ((4 * low >= 3 * cus && low <= cus) || (a.N > 64 && a.N <= 128 && a.KB >= 4 && low > cus && low <= 2 * cus))
+            return launch_tile<4, 1, 2, 4, BF16>(a, s);
         if (a.N > 64 && tiles(128, 128) >= cus / 2) return launch_tile<4, 2, 2, 4, BF16>(a, s);
     } else {
         if (a.N > 64 && tiles(128, 128) >= cus) return launch_tile<4, 4, 2, 2, BF16>(a, s);

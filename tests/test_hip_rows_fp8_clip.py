@@ -343,10 +343,15 @@ def test_product(rows, K, N, dtype):
 # many rows: (rows, K, N, bytes behind a row), for the tiles of 128 x 128 and 256 x 256, whole and odd sizes in every direction
 TILE_SIZES = [(700, 400, 70, 0), (1000, 1040, 97, 48), (6000, 256, 500, 0), (3000, 144, 60, 0), (1030, 160, 1100, 0), (1024, 512, 1024, 0), (2001, 272, 515, 16), (1030, 301, 1100, 0), (1100, 1000, 1029, 7), (8200, 16, 129, 0),
               (4100, 784, 4120, 0), (4096, 768, 4096, 0), (5000, 144, 4000, 112), (4300, 900, 4001, 3)]
+# long rows shared by few workgroups (two blocks of K under way, 16 to 64 rows to a workgroup, a short last block or none), and
+# tiles of 128 x 64
+LONG_SIZES = [(3, 8208, 333, 0), (16, 4096, 6144, 0), (16, 2064, 9000, 0), (30, 4112, 4000, 0), (40, 4112, 4000, 16), (60, 4112, 3990, 0),
+              (45, 2320, 8000, 0), (60, 2320, 7990, 0), (100, 4240, 4000, 0), (120, 8192, 1000, 0), (8100, 528, 250, 0), (24000, 528, 120, 0),
+              (20000, 1000, 100, 1)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,K,N,gap", TILE_SIZES)
+@pytest.mark.parametrize("rows,K,N,gap", TILE_SIZES + LONG_SIZES)
 def test_product_of_many_rows(rows, K, N, gap, dtype):
     xq, xs, wq, ws = (t.to(DEV) for t in _mix_inputs(rows, K, N, 6))
     bx = torch.full((rows, K + gap), 0x7f, dtype=torch.uint8, device=DEV)                      # NaN behind the rows
