@@ -1019,7 +1019,7 @@ def main():
     if os.environ.get("DSW_BENCH_NO_GRAPH") == "1":
         args.no_graph = True
     from dsw_amd import _native
-    from dsw_amd.parallel import GradBucket, init_from_env
+    from dsw_amd.parallel import GradBucket, init_from_env, settle_collectives
 
     rank, world, local = init_from_env()
     assert world == args.gpus, (world, args.gpus)
@@ -1151,6 +1151,7 @@ def main():
             sync_grads()
             torch.cuda.synchronize()
             want = bucket.bucket.clone()
+            settle_collectives()         # (the watchdog may have no event of the exchange's stream left to ask for)
             g1 = gm = None
             try:
                 # ("thread_local": RCCL's watchdog thread polls events while this thread records - an error under the default

@@ -59,6 +59,18 @@ def init_from_env(backend: str | None = None):
     return rank, world, local
 
 
+def settle_collectives(seconds: float = 0.5):
+    """Call before recording RCCL collectives into a graph.  The process group's watchdog thread asks the events of eager
+    collectives, every 100 ms, until it has seen each of them finished; while the stream they were issued on is being captured
+    that question is an error - whatever the capture mode - and ends the process.  Once the device is idle and a few of its
+    rounds have passed there is nothing left that it asks for (recorded collectives are not on its list)."""
+    import time
+
+    if dist.is_available() and dist.is_initialized() and dist.get_backend() == "nccl":
+        torch.cuda.synchronize()
+        time.sleep(seconds)
+
+
 def shard_batch(global_batch: int, rank: int, world: int):
     """Contiguous [start, stop) slice of the batch owned by ``rank`` (ragged tails allowed)."""
     base, extra = divmod(global_batch, world)

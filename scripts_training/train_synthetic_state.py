@@ -174,7 +174,11 @@ class Trainer:
             self.bucket.capturing = True      # the hooks must not enqueue collectives into the recording
             # "thread_local": RCCL's watchdog thread polls the events of the warm-up collectives (hipEventQuery) while this
             # thread records; under the default global capture mode such a call from ANOTHER thread is an error that ends the
-            # process (seen once in ~10 runs of the one-rank RCCL test: ProcessGroupNCCL watchdog abort)
+            # process (seen once in ~10 runs of the one-rank RCCL test: ProcessGroupNCCL watchdog abort); events of the
+            # stream that the recorded exchange uses must be settled before
+            from dsw_amd.parallel import settle_collectives
+
+            settle_collectives()
             mode = {"capture_error_mode": "thread_local"} if self.distributed else {}
             with torch.cuda.graph(g, **mode):
                 self.loss = self._fwd_bwd()

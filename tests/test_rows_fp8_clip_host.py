@@ -217,3 +217,19 @@ def test_layers_and_bucket_reach_the_operators():
     with pytest.raises(ValueError, match="max_norm"):
         bucket.zero()
         bucket.clip_norm(-1.0)
+
+
+def test_settling_collectives_waits_for_rccl_alone(monkeypatch):
+    """Without a process group, or with gloo (whose calls are the host's), nothing waits; with RCCL the device is idle first."""
+    from dsw_amd import parallel
+
+    seen = []
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: seen.append("idle"))
+    monkeypatch.setattr("time.sleep", lambda s: seen.append(s))
+    parallel.settle_collectives()
+    for backend, want in (("gloo", []), ("nccl", ["idle", 0.5])):
+        seen.clear()
+        monkeypatch.setattr(parallel.dist, "is_initialized", lambda: True)
+        monkeypatch.setattr(parallel.dist, "get_backend", lambda *a, b=backend: b)
+        parallel.settle_collectives()
+        assert seen == want
