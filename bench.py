@@ -981,7 +981,7 @@ def _arm_watchdog(rank, world, limit=None, what="the run", retry=False):
             # and a rank that exits takes the whole job down.  Every rank sits behind the same guard, so every rank
             # runs the next, more conservative rung in its place (same RANK / WORLD_SIZE / MASTER_*, a new process group
             # behind its own store prefix - dsw_amd.parallel.init_from_env): in a child, whose exit code becomes its own.
-            # (A process that has initialised the GPU may not be replaced by exec where the driver or a sandbox refuses it.)
+            # (A process that has initialised the GPU may not be replaced by exec everywhere.)
             print("bench.py: rank %d/%d: %s still not finished after %.0f s - re-executing with %s" % (
                 rank, world, what, limit, nxt), file=sys.stderr, flush=True)
             env = dict(os.environ, **nxt)
