@@ -6,6 +6,7 @@ parameter / buffer names (``conv1.convblock1.conv.weight``, ``conv1.rezero_weigh
 ``conv1.res_connection.weight``, ``pool1.remap_matrix`` ...) and forward semantics, so that
 checkpoints and the JSON configs of the reference load unchanged.  Pinned by fixture G5.
 """
+import weakref
 from typing import Dict
 
 import numpy as np
@@ -98,15 +99,22 @@ class _NodeLinear(Linear):
         super().__init__(*args, **kwargs)
         self._lay_out_weight()
 
-    _fp8 = None          # (Fp8Weight, the weight's version it was made from) while the 8-bit path is on
+    _fp8 = None          # (Fp8Weight, the weight it was made from (weakly), that weight's version) while the 8-bit path is on
 
     def serve_fp8(self, enable=True):
         """Inference through the 8-bit channel mix: the weight is quantised now (a scale per 128 x 128 block), the input rows
-        in each call.  Only calls under ``torch.no_grad()`` take it; moving or casting the module switches it off, and a weight
-        that has changed since raises (call it again; writes through ``weight.data`` are not noticed)."""
+        in each call.  Only calls under ``torch.no_grad()`` take it; moving, casting or copying the module switches it off, and a
+        weight that has changed since, or another tensor in its place, raises (call it again; writes through ``weight.data``
+        are not noticed)."""
         with torch.no_grad():
-            self._fp8 = (dsw_functional.quantize_fp8_weight(self.weight.t()), self.weight._version) if enable else None
+            self._fp8 = ((dsw_functional.quantize_fp8_weight(self.weight.t()), weakref.ref(self.weight), self.weight._version)
+                         if enable else None)
         return self
+
+    def __getstate__(self):
+        state = self.__dict__.copy()      # (a copy has a weight of its own)
+        state.pop("_fp8", None)
+        return state
 
     def _lay_out_weight(self):
         # only a REGISTERED parameter is re-laid, and only in place of its data: SWAG (reference modules/swag.py:33-48)
@@ -125,8 +133,8 @@ class _NodeLinear(Linear):
 
     def forward(self, x):
         if self._fp8 is not None and not torch.is_grad_enabled():
-            weight, version = self._fp8
-            if self.weight._version != version:
+            weight, made_from, version = self._fp8
+            if made_from() is not self.weight or self.weight._version != version:
                 raise RuntimeError("the weight has changed since serve_fp8(): call it again (or serve_fp8(False))")
             return dsw_functional.dense_mix_fp8(x, weight, self.bias)
         # `weight.t()` is dense [in, out] for the column-major parameter; a row-major tensor (SWAG sample, user

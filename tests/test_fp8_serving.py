@@ -1,0 +1,86 @@
+"""The residual branch's 8-bit path serves the weight that the layer has now, or raises (host logic: plain stand-ins for the quantiser
+and the product, so these run on the CPU)."""
+import copy
+import io
+
+import pytest
+import torch
+
+from dsw_amd import functional as F
+from modules import my_models_graph as M
+
+
+@pytest.fixture()
+def stand_ins(monkeypatch):
+    """The quantised weight is a copy of its values, the product an ordinary one in their precision."""
+    made = []
+
+    def quantize(weight):
+        made.append(weight)
+        return F.Fp8Weight(weight.detach().t().clone(), torch.ones(1, 1))
+
+    monkeypatch.setattr(M.dsw_functional, "quantize_fp8_weight", quantize)
+    monkeypatch.setattr(M.dsw_functional, "dense_mix_fp8", lambda x, w, bias=None: x @ w.q.t() + bias)
+    return made
+
+
+def _served(lin, x):
+    """What the layer answers under no_grad: a tensor, or None where it raises that the weight has changed."""
+    with torch.no_grad():
+        try:
+            return lin(x)
+        except RuntimeError as exc:
+            assert "has changed" in str(exc)
+            return None
+
+
+def _right(lin, x):
+    """The layer's answer is the present weight's, or it raises."""
+    y = _served(lin, x)
+    return y is None or torch.equal(y, x @ lin.weight.detach().t() + lin.bias.detach())
+
+
+def test_another_tensor_in_the_weights_place(stand_ins):
+    """Samples of an ensemble are plain tensors assigned by attribute, each of them at version 0."""
+    x = torch.randn(5, 6)
+    lin = M._NodeLinear(6, 4)
+    del lin._parameters["weight"]
+    samples = [torch.randn(4, 6) for _ in range(2)]
+    lin.weight = samples[0]
+    lin.serve_fp8()
+    assert _served(lin, x) is not None and _right(lin, x)
+    lin.weight = samples[1]
+    assert samples[0]._version == samples[1]._version and _right(lin, x)
+    lin.serve_fp8()
+    assert _served(lin, x) is not None and _right(lin, x)
+    del lin.weight                              # the tensor that it was made from dies, another one may take its place in memory
+    samples.clear()
+    lin.weight = torch.randn(4, 6)
+    assert _right(lin, x)
+
+
+def test_states_that_are_assigned(stand_ins):
+    x = torch.randn(5, 6)
+    lin = M._NodeLinear(6, 4).serve_fp8()
+    states = [{"weight": torch.randn(4, 6), "bias": torch.randn(4)} for _ in range(2)]
+    for state in states:
+        lin.load_state_dict(state, assign=True)
+        assert _right(lin, x)
+        lin.serve_fp8()
+        assert _served(lin, x) is not None and _right(lin, x)
+
+
+def test_copies_start_in_their_own_precision(stand_ins):
+    """A copy has a weight of its own: it does not inherit the switch, and copying or pickling a served layer works."""
+    x = torch.randn(5, 6)
+    lin = M._NodeLinear(6, 4).serve_fp8()
+    stand_ins.clear()
+    twin = copy.deepcopy(lin)
+    buf = io.BytesIO()
+    torch.save(lin, buf)
+    buf.seek(0)
+    for other in (twin, torch.load(buf, weights_only=False)):
+        assert other._fp8 is None and torch.equal(other.weight, lin.weight)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):        # the layer's ordinary path
+            other(x)
+    assert not stand_ins and _right(lin, x)
