@@ -99,21 +99,34 @@ class _NodeLinear(Linear):
         super().__init__(*args, **kwargs)
         self._lay_out_weight()
 
-    _fp8 = None          # (Fp8Weight, the weight it was made from (weakly), that weight's version) while the 8-bit path is on
+    _serving = None      # (the weight (weakly), its version) while the 8-bit path is on
 
     def serve_fp8(self, enable=True):
-        """Inference through the 8-bit channel mix: the weight is quantised now (a scale per 128 x 128 block), the input rows
-        in each call.  Only calls under ``torch.no_grad()`` take it; moving, casting or copying the module switches it off, and a
-        weight that has changed since, or another tensor in its place, raises (call it again; writes through ``weight.data``
-        are not noticed)."""
-        with torch.no_grad():
-            self._fp8 = ((dsw_functional.quantize_fp8_weight(self.weight.t()), weakref.ref(self.weight), self.weight._version)
-                         if enable else None)
+        """Inference through the 8-bit channel mix (weight: a scale per 128 x 128 block, rows: a scale per 128 channels).  Only
+        calls under ``torch.no_grad()`` take it; moving, casting or copying the module switches it off.  It is meant for a weight
+        at rest: one that has changed since, or another tensor in its place, raises (call it again).  What autograd does not
+        see of a weight - a replayed optimizer step, writes through ``weight.data`` - is served all the same: each call, a
+        captured one too, quantises the weight's present values (512 -> 128 channels: 23 us), and nothing of it is kept."""
+        self._serving = None
+        if enable:
+            with torch.no_grad():
+                dsw_functional.quantize_fp8_weight(self.weight.t())     # (what cannot be served raises here)
+            self._serving = (weakref.ref(self.weight), self.weight._version)
         return self
+
+    @property
+    def _fp8(self):
+        """``(Fp8Weight,)`` of the weight's present values while the 8-bit path is on, else None."""
+        if self._serving is None:
+            return None
+        weight, version = self._serving
+        if weight() is not self.weight or self.weight._version != version:
+            raise RuntimeError("the weight has changed since serve_fp8(): call it again (or serve_fp8(False))")
+        return (dsw_functional.quantize_fp8_weight(self.weight.t()),)
 
     def __getstate__(self):
         state = self.__dict__.copy()      # (a copy has a weight of its own)
-        state.pop("_fp8", None)
+        state.pop("_serving", None)
         return state
 
     def _lay_out_weight(self):
@@ -127,16 +140,13 @@ class _NodeLinear(Linear):
 
     def _apply(self, fn, *args, **kwargs):
         out = super()._apply(fn, *args, **kwargs)     # .to() / .cuda() keep dense strides; anything that did not is re-laid
-        self._fp8 = None
+        self._serving = None
         self._lay_out_weight()
         return out
 
     def forward(self, x):
-        if self._fp8 is not None and not torch.is_grad_enabled():
-            weight, made_from, version = self._fp8
-            if made_from() is not self.weight or self.weight._version != version:
-                raise RuntimeError("the weight has changed since serve_fp8(): call it again (or serve_fp8(False))")
-            return dsw_functional.dense_mix_fp8(x, weight, self.bias)
+        if self._serving is not None and not torch.is_grad_enabled():
+            return dsw_functional.dense_mix_fp8(x, self._fp8[0], self.bias)
         # `weight.t()` is dense [in, out] for the column-major parameter; a row-major tensor (SWAG sample, user
         # assignment) is made contiguous inside dense_mix - same values either way
         # (the parameter's gradient buffer, if a GradBucket in direct mode attached one: memory order [in][out], which is

@@ -84,3 +84,73 @@ def test_copies_start_in_their_own_precision(stand_ins):
         with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):        # the layer's ordinary path
             other(x)
     assert not stand_ins and _right(lin, x)
+
+
+def test_writes_that_autograd_does_not_see(stand_ins):
+    """Writes through ``weight.data`` (a replayed optimizer step is one, too) leave the version as it is: what is served is the
+    weight as it is now."""
+    x = torch.randn(5, 6)
+    lin = M._NodeLinear(6, 4).serve_fp8()
+    before = _served(lin, x)
+    lin.weight.data.mul_(3.0)
+    assert _right(lin, x) and not torch.equal(_served(lin, x), before)
+    with torch.no_grad():
+        lin.weight.add_(1.0)
+    assert _served(lin, x) is None                                # autograd's own count: raises, as promised
+    assert _right(lin.serve_fp8(), x) and _served(lin, x) is not None
+
+
+def _alike(a, b):
+    return a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_a_replayed_update_reaches_the_served_weight():
+    """serve_fp8 - an optimizer step that is replayed from a graph - inference: the new weight's values."""
+    torch.manual_seed(0)
+    lin = M._NodeLinear(200, 72).to("cuda")
+    x, new = torch.randn(90, 200, device="cuda"), torch.randn(72, 200, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.no_grad():
+        lin.weight.add_(new)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    update = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(update), torch.no_grad():
+        lin.weight.add_(new)
+    lin.serve_fp8()
+    for _ in range(3):
+        update.replay()
+        with torch.no_grad():
+            y = lin(x)
+            want = F.dense_mix_fp8(x, F.quantize_fp8_weight(lin.weight.t()), lin.bias)
+        torch.cuda.synchronize()
+        assert _alike(y, want)
+
+
+@pytest.mark.gpu
+def test_captured_inference_follows_the_weight():
+    """A captured inference graph answers with the weight at each replay, whatever is done with the switch in between."""
+    torch.manual_seed(0)
+    lin = M._NodeLinear(130, 72).to("cuda").serve_fp8()
+    x = torch.randn(90, 130, device="cuda")
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            lin(x)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = lin(x)
+        for step in range(4):
+            lin.weight.mul_(-1.5)
+            if step % 2 == 0:
+                lin.serve_fp8(step == 0)                      # again, and off: the graph's own memory is not theirs
+            trash = [torch.full((72, 130), 7, dtype=torch.uint8, device="cuda") for _ in range(8)]
+            graph.replay()
+            torch.cuda.synchronize()
+            assert _alike(y, F.dense_mix_fp8(x, F.quantize_fp8_weight(lin.weight.t()), lin.bias))
+            assert all(bool((t == 7).all()) for t in trash)
