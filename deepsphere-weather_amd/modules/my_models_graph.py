@@ -124,6 +124,10 @@ class _NodeLinear(Linear):
             raise RuntimeError("the weight has changed since serve_fp8(): call it again (or serve_fp8(False))")
         return (dsw_functional.quantize_fp8_weight(self.weight.t()),)
 
+    def serves_fp8(self):
+        """Whether a call now takes the 8-bit path."""
+        return self._serving is not None and not torch.is_grad_enabled()
+
     def __getstate__(self):
         state = self.__dict__.copy()      # (a copy has a weight of its own)
         state.pop("_serving", None)
@@ -145,7 +149,7 @@ class _NodeLinear(Linear):
         return out
 
     def forward(self, x):
-        if self._serving is not None and not torch.is_grad_enabled():
+        if self.serves_fp8():
             return dsw_functional.dense_mix_fp8(x, self._fp8[0], self.bias)
         # `weight.t()` is dense [in, out] for the column-major parameter; a row-major tensor (SWAG sample, user
         # assignment) is made contiguous inside dense_mix - same values either way
@@ -212,6 +216,8 @@ class ResBlock(torch.nn.Module):
             return False
         if not isinstance(self.res_connection, (_NodeLinear, Identity)):
             return False
+        if isinstance(self.res_connection, _NodeLinear) and self.res_connection.serves_fp8():
+            return False     # the shortcut multiplies by the branch's weight itself
         return x.dtype == torch.float32
 
     def forward(self, x, out=None):

@@ -100,6 +100,55 @@ def test_writes_that_autograd_does_not_see(stand_ins):
     assert _right(lin.serve_fp8(), x) and _served(lin, x) is not None
 
 
+def _block(cin, widths):
+    from dsw_amd import sphere
+    from modules.layers import prepare_torch_laplacian
+
+    lap = prepare_torch_laplacian(sphere.SphereHealpix(4, nest=True, k=8).L, lmax=1.9)
+    opts = dict(kernel_size=3, conv_type="graph", bias=True, batch_norm=False, batch_norm_before_activation=False,
+                activation=True, activation_fun="relu", periodic_padding=True, lonlat_ratio=None)
+    return M.ResBlock(cin, widths, laplacian=lap, convblock_kwargs=opts)
+
+
+def test_a_block_with_a_fused_tail_serves_its_branch(stand_ins, oracle_backend, monkeypatch):
+    """Where the last convolution would take the block's tail and read the branch's weight itself, the switch decides."""
+    monkeypatch.setattr(M.ResBlock, "fuse_tail", True)
+    block, x = _block(6, (12, 10)), torch.randn(2, 192, 6)
+    with torch.no_grad():
+        plain = block(x)
+        assert block._fusable_tail(x) and M.serve_fp8(block) == 1
+        stand_ins.clear()
+        y = block(x)
+        assert len(stand_ins) == 1 and float((y - plain).abs().max()) <= 1e-5 * float(plain.abs().max())
+        block.res_connection.weight.add_(1.0)
+        with pytest.raises(RuntimeError, match="has changed"):
+            block(x)
+        M.serve_fp8(block)
+    assert block._fusable_tail(x)                               # with gradients the layer is what it was
+    stand_ins.clear()
+    block(x.requires_grad_()).sum().backward()
+    assert not stand_ins and block.res_connection.weight.grad is not None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fuse_tail", [False, True])
+def test_every_served_branch_takes_the_8_bit_product(fuse_tail, monkeypatch):
+    """One 8-bit product for each branch that serve_fp8 counts, as the library's launch trace sees them."""
+    from dsw_amd import _native
+
+    monkeypatch.setattr(M.ResBlock, "fuse_tail", fuse_tail)
+    blocks = [_block(18, (64, 128)), _block(128, (64, 32)), _block(32, (32,)), _block(32, 2)]
+    model = torch.nn.Sequential(*blocks).to("cuda").eval()
+    x = torch.randn(2, 192, 18, device="cuda")
+    with torch.no_grad():
+        model(x)
+        found = M.serve_fp8(model)
+        with _native.LaunchTrace() as trace:
+            model(x)
+            torch.cuda.synchronize()
+    assert found == 3 and [r[1:4] for r in trace.intervals if r[0] == "fp8_mix"] == [(384, 18, 128), (384, 128, 32), (384, 32, 2)]
+
+
 def _alike(a, b):
     return a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
 
