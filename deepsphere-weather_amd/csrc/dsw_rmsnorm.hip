@@ -88,12 +88,13 @@ __global__ __launch_bounds__(RN_THREADS) void rmsnorm_fwd_kernel(const NormArgs 
                 a = j < n && b > a ? b : a;
             }
             a = lanes_umax<128 / V>(a);
-            const float s = e4m3_scale(a), inv = e4m3_inverse(s);
+            const float s = e4m3_scale(a);
             if (n > 0) {
+                float z[V];
+                e4m3_quotients(v[i], s, z);
                 uint32_t q[V / 4];
 #pragma unroll
-                for (int j = 0; j < V / 4; ++j)
-                    q[j] = e4m3_pack4(v[i][4 * j] * inv, v[i][4 * j + 1] * inv, v[i][4 * j + 2] * inv, v[i][4 * j + 3] * inv);
+                for (int j = 0; j < V / 4; ++j) q[j] = e4m3_pack4(z[4 * j], z[4 * j + 1], z[4 * j + 2], z[4 * j + 3]);
                 uint8_t* out = P.Q + row * P.C + c;
                 if (n >= V) {
                     struct __attribute__((packed, aligned(1))) Bytes { uint32_t q[V / 4]; } b;
@@ -169,12 +170,14 @@ __global__ __launch_bounds__(RN_THREADS) void rmsnorm_fwd_long_kernel(const Norm
                 a = j < n && b > a ? b : a;
             }
             a = lanes_umax<128 / V>(a);
-            const float s = e4m3_scale(a), inv = e4m3_inverse(s);
+            const float s = e4m3_scale(a);
             if (n > 0) {
                 uint8_t* out = P.Q + row * P.C + c;
+                float z[V];
+                e4m3_quotients(v, s, z);
 #pragma unroll
                 for (int j = 0; j < V; j += 4) {
-                    const uint32_t q = e4m3_pack4(v[j] * inv, v[j + 1] * inv, v[j + 2] * inv, v[j + 3] * inv);
+                    const uint32_t q = e4m3_pack4(z[j], z[j + 1], z[j + 2], z[j + 3]);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) if (j + k < n) out[j + k] = (uint8_t)(q >> (8 * k));
                 }
@@ -490,12 +493,14 @@ __global__ __launch_bounds__(1024) void quant_weight_kernel(const char* W, long 
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < 16; ++q) a = red[q] > a ? red[q] : a;
-    const float s = e4m3_scale(a), inv = e4m3_inverse(s);
+    const float s = e4m3_scale(a);
     if (threadIdx.x == 0) S[(long)blockIdx.y * KB + blockIdx.x] = s;
+    float z[EACH];
+    e4m3_quotients(v, s, z);
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         const int n = along_n ? lo : hi + 8 * i, k = along_n ? hi + 8 * i : lo;
-        tile[n * PITCH + k] = (uint8_t)e4m3_pack4(v[i] * inv, 0.f, 0.f, 0.f);
+        tile[n * PITCH + k] = (uint8_t)e4m3_pack4(z[i], 0.f, 0.f, 0.f);
     }
     __syncthreads();
     const int n = threadIdx.x >> 3, k = (threadIdx.x & 7) * 16;
