@@ -16,6 +16,7 @@
 
 #include <array>
 #include <cmath>
+#include <functional>
 #include <optional>
 #include <string>
 #include <vector>
@@ -369,6 +370,10 @@ Tensor grad_norm_clip(std::vector<Tensor> grads, const std::optional<std::vector
             TORCH_CHECK_VALUE(dense(to[i]), "dsw: a clipped tensor must be dense (cover consecutive elements, in any dimension order)");
         }
     }
+    if (at::GradMode::is_enabled())
+        for (const auto& list : {std::cref(grads), std::cref(to)})
+            for (const Tensor& t : list.get())
+                TORCH_CHECK(!wants_grad(t), "dsw: the gradient norm and the clipping have no backward pass; call them under torch.no_grad() or detach() the tensors");
     on_gpu(grads[0]);
     const c10::DeviceGuard guard(dev);
     const at::AutoGradMode off(false);

@@ -1326,7 +1326,8 @@ def dense_mix_fp8(x, weight: Fp8Weight, bias: torch.Tensor = None, dtype: torch.
 
 def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     """Norm (1, 2 or inf) of all ``tensors`` taken together (fp32 and bf16, mixed, any shapes), a 0-dim fp32 tensor on their
-    device.  Two launches for up to 144 tensors (a flat bucket's views count as one); sums in 64 bits; capturable."""
+    device.  Two launches for up to 144 tensors (a flat bucket's views count as one), one more for each further 144; sums in 64 bits;
+    capturable.  No backward: with autograd on, tensors that require a gradient are refused (``detach()`` them)."""
     return _native.ops().grad_norm_clip([tensors] if isinstance(tensors, torch.Tensor) else list(tensors), None, norm_type, 0.0, False)
 
 
@@ -1334,7 +1335,8 @@ def clip_grad_norm_(tensors, max_norm: float, norm_type: float = 2.0, out=None) 
     """Scale ``tensors`` by ``min(1, max_norm / (norm + 1e-6))`` with their common norm and return that norm (0-dim fp32, on the
     device: nothing is read back).  In place, or into ``out`` (a tensor of the same shape and type for each).  A tensor listed
     twice, or one that overlaps another one of the call, is refused.  A norm that is not finite behaves as the formula does:
-    an infinite one gives zeros (and NaN in its infinite places), a NaN gives NaN."""
+    an infinite one gives zeros (and NaN in its infinite places), a NaN gives NaN.  No backward: with autograd on, tensors that
+    require a gradient are refused, as torch refuses to write over them (``torch.no_grad()``, or ``detach()``)."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if out is not None:
         out = [out] if isinstance(out, torch.Tensor) else list(out)
