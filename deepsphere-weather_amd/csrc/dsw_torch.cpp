@@ -72,7 +72,14 @@ void on_gpu(const Tensor& t) {
 }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+// (a result without a tangent would read as a derivative of zero; no_grad does not switch tangents off)
+void no_tangent(std::initializer_list<const Tensor*> tensors) {
+    for (const Tensor* t : tensors)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "dsw: the row norm, the 8-bit channel mix and the gradient norm have no "
+                    "forward-mode derivative; unpack the dual tensor (torch.autograd.forward_ad.unpack_dual)");
+}
 void no_backward(const char* what, std::initializer_list<const Tensor*> tensors) {
+    no_tangent(tensors);
     if (!at::GradMode::is_enabled()) return;
     for (const Tensor* t : tensors)
         TORCH_CHECK(!wants_grad(*t), "dsw: ", what, " is a serving path without a backward pass; call it under torch.no_grad()");
@@ -118,6 +125,7 @@ void check_norm(const Tensor& x, const Tensor& r, const Tensor& w, double eps) {
     TORCH_CHECK_VALUE(!r.defined() || r.sizes() == x.sizes(), "expected a residual of the shape of x");
     TORCH_CHECK_VALUE(eps >= 0.0 && std::isfinite(eps), "eps must be a finite number >= 0");
     code_of(x.scalar_type());
+    no_tangent({&x, &r, &w});
     same_type(x, w);
     same_device(x, w);
     if (r.defined()) { same_type(x, r); same_device(x, r); }
@@ -370,10 +378,11 @@ Tensor grad_norm_clip(std::vector<Tensor> grads, const std::optional<std::vector
             TORCH_CHECK_VALUE(dense(to[i]), "dsw: a clipped tensor must be dense (cover consecutive elements, in any dimension order)");
         }
     }
-    if (at::GradMode::is_enabled())
-        for (const auto& list : {std::cref(grads), std::cref(to)})
-            for (const Tensor& t : list.get())
-                TORCH_CHECK(!wants_grad(t), "dsw: the gradient norm and the clipping have no backward pass; call them under torch.no_grad() or detach() the tensors");
+    for (const auto& list : {std::cref(grads), std::cref(to)})
+        for (const Tensor& t : list.get()) {
+            no_tangent({&t});
+            TORCH_CHECK(!at::GradMode::is_enabled() || !wants_grad(t), "dsw: the gradient norm and the clipping have no backward pass; call them under torch.no_grad() or detach() the tensors");
+        }
     on_gpu(grads[0]);
     const c10::DeviceGuard guard(dev);
     const at::AutoGradMode off(false);
