@@ -28,6 +28,7 @@ import argparse
 import json
 import os
 import sys
+import threading
 import time
 
 REPO = os.path.dirname(os.path.abspath(__file__))
@@ -956,6 +957,11 @@ def roofline_target(args, model, x, B, V, device):
     return rl_layer, rl_what, rl_x, tkey
 
 
+HUNG = 75          # exit code of a rung whose guard fired: its supervisor starts the next one
+_line_lock = threading.Lock()
+_line_out = False  # the result line is printed: nothing may measure again
+
+
 def _next_rung():
     """Environment of the next, more conservative way to run the N > 1 step (the ladder of `launch_ranks`), or None at its end."""
     if os.environ.get("DSW_BENCH_NO_GRAPH") == "1":
@@ -965,40 +971,92 @@ def _next_rung():
     return {"DSW_BENCH_COLLECTIVES": "eager"}
 
 
+def print_line(out):
+    """Print the result; a guard that fires from here on ends the process without another attempt."""
+    global _line_out
+    with _line_lock:
+        print(json.dumps(out), flush=True)
+        _line_out = True
+
+
 def _arm_watchdog(rank, world, limit=None, what="the run", retry=False):
     """A rank of an N > 1 run that is still alive after DSW_BENCH_TIMEOUT seconds (a collective that never completes)
-    exits with an error instead of holding the node: the launcher (ours, or torchrun) then tears the job down.  Also
-    used with a short limit around the FIRST replay of a graph that holds collectives."""
-    import threading
-
+    exits with an error instead of holding the node: its supervisor (``retry``) runs the next rung of the ladder, any other launcher
+    tears the job down.  Also used with a short limit around the FIRST replay of a graph that holds collectives."""
     if limit is None:
-        limit = float(os.environ.get("DSW_BENCH_TIMEOUT", "420")) * 0.9
+        limit = _run_limit()
 
     def bark():
-        nxt = _next_rung()
-        if retry and nxt is not None:
-            # launched by somebody else's torchrun (the driver's scaling run): nobody will start a second attempt for us,
-            # and a rank that exits takes the whole job down.  Every rank sits behind the same guard, so every rank
-            # runs the next, more conservative rung in its place (same RANK / WORLD_SIZE / MASTER_*, a new process group
-            # behind its own store prefix - dsw_amd.parallel.init_from_env): in a child, whose exit code becomes its own.
-            # (A process that has initialised the GPU may not be replaced by exec everywhere.)
-            print("bench.py: rank %d/%d: %s still not finished after %.0f s - re-executing with %s" % (
-                rank, world, what, limit, nxt), file=sys.stderr, flush=True)
-            env = dict(os.environ, **nxt)
-            env["DSW_PG_ATTEMPT"] = str(int(os.environ.get("DSW_PG_ATTEMPT", "0") or 0) + 1)
+        with _line_lock:                 # (never while the line is being printed; whichever timer is first ends the process)
+            again = retry and not _line_out and _next_rung() is not None
+            print("bench.py: rank %d/%d: %s still not finished after %.0f s - %s" % (
+                rank, world, what, limit, "leaving it to the next rung" if again else "giving up"), file=sys.stderr, flush=True)
             sys.stdout.flush()
-            import subprocess
-
-            rc = subprocess.call([sys.executable, os.path.abspath(__file__), *sys.argv[1:]], env=env)
-            os._exit(rc if rc >= 0 else 128 - rc)
-        print("bench.py: rank %d/%d: %s still not finished after %.0f s - giving up" % (rank, world, what, limit),
-              file=sys.stderr, flush=True)
-        os._exit(124)
+            os._exit(HUNG if again else 124)
 
     t = threading.Timer(limit, bark)
     t.daemon = True
     t.start()
     return t
+
+
+def _run_limit():
+    return float(os.environ.get("DSW_BENCH_TIMEOUT", "420")) * 0.9
+
+
+def _die_with_supervisor():
+    """A rung ends with the process that started it, however that one ends."""
+    import ctypes
+    import signal
+
+    ctypes.CDLL(None).prctl(1, signal.SIGKILL)                           # PR_SET_PDEATHSIG
+    if os.getppid() != int(os.environ.pop("DSW_BENCH_SUPERVISOR")):      # it ended before the line above (popped: not for children)
+        os._exit(124)
+
+
+def supervise(command):
+    """Rank of an N > 1 run under somebody else's launcher (torchrun): nobody starts a second attempt for us, and a rank that exits takes
+    the whole job down.  So the rank's own process stays off the GPU and runs the step in a child (same RANK / WORLD_SIZE /
+    MASTER_*); a child whose guard fired is gone, with its collectives, before the next, more conservative rung starts in a new
+    process group behind its own store prefix (dsw_amd.parallel.init_from_env).  Every rank sits behind the same guards, so
+    all of them take that step together.  Returns the exit code."""
+    import signal
+    import subprocess
+
+    child = None
+
+    def stop(signum, frame):
+        if child is not None and child.poll() is None:
+            child.terminate()
+            try:
+                child.wait(10)
+            except subprocess.TimeoutExpired:
+                child.kill()
+        os._exit(128 + signum)
+
+    for s in (signal.SIGTERM, signal.SIGINT, signal.SIGHUP):
+        signal.signal(s, stop)
+    os.environ["DSW_BENCH_SUPERVISOR"] = str(os.getpid())
+    while True:
+        child = subprocess.Popen(command)
+        try:
+            rc = child.wait(_run_limit() + 60)
+        except subprocess.TimeoutExpired:                                # (its own guards could not end it)
+            child.kill()
+            try:
+                child.wait(30)
+            except subprocess.TimeoutExpired:
+                return 124
+            rc = HUNG
+        if rc != HUNG:
+            return rc if rc >= 0 else 128 - rc
+        nxt = _next_rung()
+        if nxt is None:
+            return 124
+        print("bench.py: rank %s/%s: re-executing in a new process with %s" % (
+            os.environ.get("RANK", "0"), os.environ.get("WORLD_SIZE", "1"), nxt), file=sys.stderr, flush=True)
+        os.environ.update(nxt)
+        os.environ["DSW_PG_ATTEMPT"] = str(int(os.environ.get("DSW_PG_ATTEMPT", "0") or 0) + 1)
 
 
 def main():
@@ -1016,6 +1074,12 @@ def main():
         sys.exit(launch_ranks(args.gpus, sys.argv[1:]))
     if env_world is not None and int(env_world) != args.gpus:
         sys.exit("bench.py: --gpus %d but the launcher started %s rank(s) (WORLD_SIZE)" % (args.gpus, env_world))
+    supervised = "DSW_BENCH_SUPERVISOR" in os.environ
+    if supervised:
+        _die_with_supervisor()
+    elif env_world is not None and not os.environ.get("DSW_BENCH_LAUNCHER") and (
+            args.gpus > 1 or os.environ.get("DSW_FORCE_GRAD_SYNC") == "1"):
+        sys.exit(supervise([sys.executable, os.path.abspath(__file__), *sys.argv[1:]]))
     if os.environ.get("DSW_BENCH_NO_GRAPH") == "1":
         args.no_graph = True
     from dsw_amd import _native
@@ -1023,9 +1087,9 @@ def main():
 
     rank, world, local = init_from_env()
     assert world == args.gpus, (world, args.gpus)
-    # ranks started by somebody else's launcher (the driver's torchrun) climb down the ladder in place (see `_arm_watchdog`);
-    # under our own self-launch the launcher process does (launch_ranks)
-    external = os.environ.get("WORLD_SIZE") is not None and not os.environ.get("DSW_BENCH_LAUNCHER")
+    # ranks started by somebody else's launcher climb down the ladder under their supervisor; under our own self-launch the
+    # launcher process does (launch_ranks)
+    external = supervised
     if world > 1:
         _arm_watchdog(rank, world, retry=external)
     assert torch.cuda.is_available(), "bench.py measures the HIP path; a ROCm device is required"
@@ -1308,8 +1372,8 @@ def main():
     if os.environ.get("DSW_BENCH_LAUNCHER"):
         out["config"]["launcher"] = os.environ["DSW_BENCH_LAUNCHER"]
     if os.environ.get("DSW_PG_ATTEMPT"):
-        out["config"]["ladder"] = ("rung %d of the in-place fallback ladder (a guard fired in the rung before: the ranks re-executed "
-                                   "themselves under the same launcher)" % (int(os.environ["DSW_PG_ATTEMPT"]) + 1))
+        out["config"]["ladder"] = ("rung %d of the in-place fallback ladder (a guard fired in the rung before: the ranks ran the step "
+                                   "again in new processes under the same launcher)" % (int(os.environ["DSW_PG_ATTEMPT"]) + 1))
     if os.environ.get("DSW_HIP_LIB"):
         out["config"]["DSW_HIP_LIB"] = os.environ["DSW_HIP_LIB"]   # an A/B build stands in for the product library
     if bucket.active():
@@ -1427,7 +1491,7 @@ def main():
             else:
                 out["cpu_baseline"] = cpu_baseline_leg(wl, lap, model)
     if rank == 0:
-        print(json.dumps(out), flush=True)
+        print_line(out)
     if world > 1:
         dist.barrier()
         dist.destroy_process_group()

@@ -39,10 +39,10 @@ def init_from_env(backend: str | None = None):
         kw = {}
         attempt = int(os.environ.get("DSW_PG_ATTEMPT", "0") or 0)
         if attempt > 0:
-            # A rank that re-executed itself (bench.py: the first replay of a graph-captured exchange never came back) joins a
+            # A rank whose step is run again (bench.py: the first replay of a graph-captured exchange never came back) joins a
             # NEW process group under the same launcher: the launcher's store still holds the keys of the first group
             # (barrier counts, the communicator id), so this incarnation talks through its own key prefix.  Under torchrun
-            # the agent hosts the store; without it rank 0 does (and its old store died with the old process image).
+            # the agent hosts the store; without it rank 0 does (and its old store died with the old process).
             from datetime import timedelta
 
             agent_store = os.environ.get("TORCHELASTIC_USE_AGENT_STORE") == "True"
