@@ -59,15 +59,24 @@ def init_from_env(backend: str | None = None):
     return rank, world, local
 
 
+def _process_groups():
+    """The process groups of this process, the default one among them."""
+    return list(dist.distributed_c10d._world.pg_map)
+
+
 def settle_collectives(seconds: float = 0.5):
     """Call before recording RCCL collectives into a graph.  The process group's watchdog thread asks the events of eager
     collectives, every 100 ms, until it has seen each of them finished; while the stream they were issued on is being captured
-    that question is an error - whatever the capture mode - and ends the process.  Once the device is idle and a few of its
-    rounds have passed there is nothing left that it asks for (recorded collectives are not on its list)."""
+    that question is an error - whatever the capture mode - and ends the process.  So the device is idle first, and then every
+    group has let go of the last collective on its list (``_wait_for_pending_works``: back at once when there is none, else with
+    the watchdog's next round; recorded collectives are not on that list).  ``seconds``: for what else its threads may be at."""
     import time
 
     if dist.is_available() and dist.is_initialized() and dist.get_backend() == "nccl":
         torch.cuda.synchronize()
+        for group in _process_groups():
+            if dist.get_backend(group) == "nccl":
+                group._wait_for_pending_works()
         time.sleep(seconds)
 
 
