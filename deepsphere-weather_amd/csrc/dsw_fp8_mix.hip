@@ -666,15 +666,17 @@ static int64_t mix_ws_bytes(int64_t M, int64_t N, int64_t K, bool aligned) {
 //   98304 x 256 x 64      38.8    10.8     11.2     17.6
 //   4096 x 512 x 4096     99.8    30.8     19.1     17.9
 //   4096 x 4096 x 4096   294     144       78.1     62.6
-// as long as the LDS kernel's workgroups come to four per CU - that; 128 x 128 as soon as there is such a tile for every other CU
-// (and more than 64 outputs), 256 x 256 as soon as there is one for every CU (from four blocks of K on: below, its fuller
+// as long as the LDS kernel's workgroups come to four per CU - that; 32 x 128 up to 64 outputs; 128 x 128 as soon as there is such a
+// tile for every other CU, 256 x 256 as soon as there is one for every CU (from four blocks of K on: below, its fuller
 // epilogue costs more than it saves) and they cover at most a quarter more than 128 x 128 does.  Between them 128 x 64, three to a CU,
-// where they are at most one for every CU, or two over a single column of tiles (rows are read once either way):
-//   rows x K x N         128 x 64   else             rows x K x N         128 x 64   128 x 128   256 x 256
-//   8192 x 512 x 256        4.9      5.5             24576 x 512 x 128       7.0       7.6
-//   5000 x 1024 x 384       7.5      9.3             98304 x 512 x 128      19.4      17.8         25.0
-//   4096 x 4096 x 512      21.0     24.6             49152 x 1024 x 300     34.4      30.7         36.0
-//   6000 x 512 x 512        6.6      6.0             20000 x 4096 x 640     87.3      73.5         74.5
+// from three for four CUs up to two for each; operands of the call before (in the caches) / of ten calls in turn:
+//   rows x K x N          32 x 128      128 x 64     128 x 128       rows x K x N          32 x 128      128 x 64     128 x 128
+//   8192 x 512 x 250      5.7 / 7.5     5.0 / 7.4    6.0 / 8.4       30000 x 512 x 128     8.7 / 12.5    6.6 / 8.7    6.2 / 9.2
+//   16384 x 512 x 128     5.4 / 7.2     4.8 / 7.4    5.5 / 8.0       24576 x 2048 x 128   17.3 / 24.4   15.0 / 21.2  16.7 / 21.7
+//   24576 x 512 x 128     6.7 / 8.4     6.3 / 8.5    5.8 / 8.6       6000 x 512 x 512      6.6 / 8.2     6.2 / 8.2    5.8 / 8.2
+//   24576 x 640 x 80      6.8 / 8.5     6.4 / 8.8    5.9 / 9.2       12000 x 1024 x 256      - / 11.0      - / 10.7     - / 10.8
+//   4096 x 4096 x 512    24.7 / -      20.4 / -     24.1 / -         22000 x 1024 x 128      - / 11.3      - / 10.7     - / 11.5
+//   16384 x 512 x 64      4.3 / 6.2     4.4 / 7.1    5.2 / 7.8       24576 x 1024 x 64     6.9 / 10.4    7.8 / 10.4   7.1 / 11.6
 // fp32 output (bf16 matrix instructions): 128 x 128 by four waves instead of eight (4096^3: 139 against 154) from one for every CU
 // on (6000 x 512 x 512: 11.3 against 10.1 of the 32 x 128), no larger ones.
 template <bool BF16>
@@ -699,8 +701,7 @@ static int launch_mix(const MixArgs& a, hipStream_t s) {
     if constexpr (BF16) {
         if (a.KB >= 4 && tiles(256, 256) >= cus && 16 * tiles(256, 256) <= 5 * tiles(128, 128)) return launch_tile<8, 4, 2, 4, BF16>(a, s);
         const long low = tiles(128, 64);
-        if ((4 * low >= 3 * cus && low <= cus) || (a.N > 64 && a.N <= 128 && a.KB >= 4 && low > cus && low <= 2 * cus))
-            return launch_tile<4, 1, 2, 4, BF16>(a, s);
+        if (a.N > 64 && 4 * low >= 3 * cus && low <= 2 * cus) return launch_tile<4, 1, 2, 4, BF16>(a, s);
         if (a.N > 64 && tiles(128, 128) >= cus / 2) return launch_tile<4, 2, 2, 4, BF16>(a, s);
     } else {
         if (a.N > 64 && tiles(128, 128) >= cus) return launch_tile<4, 4, 2, 2, BF16>(a, s);
