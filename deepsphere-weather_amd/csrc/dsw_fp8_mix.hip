@@ -637,22 +637,34 @@ static int64_t mix_ws_bytes(int64_t M, int64_t N, int64_t K, bool aligned) {
     return aligned || M <= MIX_FEW_ROWS ? 0 : (M + N) * ((K + 15) / 16 * 16);
 }
 
-// Which kernel, aligned rows (times in us, bf16 output).  Few rows or outputs: the LDS kernel, named by its row tiles m, output tiles n
-// and blocks of a wave under way:
-//   rows x K x N        registers  1,1,1  1,1,2  2,1,1  2,1,2  3,1,1  4,1,2  4,2,1
-//   1 x 4096 x 4096         5.3     5.7    5.0
-//   16 x 8192 x 1024       10.1     7.5    6.1
-//   16 x 8192 x 8192       17.6    12.7   13.6
-//   17 x 4096 x 4096                6.7           6.8    5.8    7.3    6.7    9.1
-//   64 x 2048 x 1024                              3.6    3.7    4.2    4.9    7.9
-//   64 x 4096 x 2048                6.3           6.5    5.5    6.9    7.0   10.9
-//   48 x 8192 x 8192                             23.6   30.2   17.8   20.5   20.7
-//   128 x 4096 x 2048               9.0           8.4    9.4    8.8    7.4   11.2
-//   128 x 4096 x 4096              16.5          15.1   18.7   15.5   14.7   12.2
-//   90 x 2304 x 4096                8.2           7.1           7.0           9.1
-// so, with at least three blocks of K for a wave: two blocks under way and as few row tiles as leave no CU a second workgroup (they
-// would not fit next to each other); else all rows in one tile up to 64 of them.  With fewer blocks small workgroups of one
-// block under way, four to a CU.
+// Which kernel, aligned rows (times in us of a replayed graph, bf16 output).  Few rows or outputs: the LDS kernel, named by its row tiles
+// m, output tiles n and blocks of a wave under way:
+//   rows x K x N          1,1,1  1,1,2  2,1,1  2,1,2  3,1,1  3,1,2  4,1,1  4,1,2  4,2,1
+//   16 x 2048 x 4096        3.2    3.2
+//   16 x 4096 x 4096        5.1    4.5
+//   16 x 8192 x 4096        7.9    6.8
+//   16 x 8192 x 6144       10.8   10.6
+//   16 x 8192 x 8192       12.8   13.5
+//   32 x 2048 x 4096                      3.8    3.8    4.2    4.2    4.5    4.6    6.3
+//   32 x 4096 x 4096                      6.1    5.4    6.5    5.8    7.0    6.3    9.0
+//   32 x 4096 x 8192                      8.8    9.6    9.5   10.3   10.4   11.2    9.7
+//   33 x 4096 x 4096                      7.3    8.4    6.9    6.1    7.4    6.5    9.1
+//   48 x 8192 x 4096                     12.0   14.4   11.3   10.1   12.0   10.7   15.1
+//   48 x 4096 x 6144                     10.2   12.0    9.3   10.6   10.2   11.4   10.2
+//   48 x 8192 x 8192                     23.6   30.1   17.8   19.4   19.0   20.4   20.5
+//   64 x 4096 x 4096                      8.8    9.5    9.3   10.7    8.7    7.8   11.1
+//   64 x 8192 x 4096                     13.0   15.1   14.3   16.8   13.1   11.9   16.6
+//   64 x 8192 x 6144                     17.7   23.1   23.7   25.6   19.4   21.1   22.2
+//   64 x 8192 x 8192                     24.9   31.4   29.4   34.1   20.8   22.1   22.0
+//   128 x 4096 x 2048                     7.6    8.5    8.0    9.4    6.9    6.7   10.1
+//   128 x 2176 x 4096                     9.0   11.6    9.7   11.3    8.5    9.7    8.9
+//   128 x 4096 x 4096                    13.7   17.2   14.2   16.1   12.7   13.9   11.4
+//   128 x 8192 x 4096                    22.3   28.9   22.6   26.3   19.3   22.0   17.8
+// so, from three blocks of K for a wave on (more than 16): two blocks under way and as few row tiles as leave no CU a second workgroup
+// (up to 16 rows, whose tiles are small enough to share one: up to three for two CUs); else, from 33 to 64 rows, all of them
+// in one tile up to two workgroups a CU (at one and a half, 64 rows would be 9 % faster in tiles of 32; at two they are 16 %
+// slower); from 32 blocks on (at 17 it is even) four row tiles and two output tiles where that leaves no CU a second
+// workgroup.  With fewer blocks two under way gain nothing: small workgroups of one, four to a CU.
 //
 // Then tiles by outputs n x rows m ("LDS": 2,1,1):
 //   rows x K x N          LDS   32x128  128x128  256x256
@@ -688,7 +700,7 @@ static int launch_mix(const MixArgs& a, hipStream_t s) {
         if (a.M <= 32) return launch_few<2, 1, 1, 8, BF16>(a, s);
         return launch_few<4, 1, 1, 8, BF16>(a, s);
     }
-    if (a.M <= 16) return a.KB > 8 && 2 * tiles(16, 16) <= 3 * cus ? launch_few_lds<1, 1, 8, 2, BF16>(a, s) : launch_few_lds<1, 1, 8, 1, BF16>(a, s);
+    if (a.M <= 16) return a.KB > 16 && 2 * tiles(16, 16) <= 3 * cus ? launch_few_lds<1, 1, 8, 2, BF16>(a, s) : launch_few_lds<1, 1, 8, 1, BF16>(a, s);
     if (a.KB > 16) {
         if (tiles(16, 32) <= cus) return launch_few_lds<2, 1, 8, 2, BF16>(a, s);
         if (tiles(16, 48) <= cus) return launch_few_lds<3, 1, 8, 2, BF16>(a, s);
