@@ -354,7 +354,8 @@ class GradBucket:
                 raise RuntimeError("GradBucket: a parameter's gradient is no longer in the bucket (zero_grad(set_to_none=True)?); "
                                    "zero() puts it back")
             return functional.clip_grad_norm_(self.bucket, max_norm, norm_type)
-        return functional.clip_grad_norm_([p.grad for p in self.params if p.grad is not None], max_norm, norm_type)
+        grads = [p.grad for p in self.params if p.grad is not None]
+        return functional.clip_grad_norm_(grads or self.bucket[:0], max_norm, norm_type)      # (without any: a norm of zero)
 
     # ---- detached mode (gradients are ordinary tensors: copy in, exchange, copy out)
     def _pack(self):
