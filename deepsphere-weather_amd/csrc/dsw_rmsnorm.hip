@@ -584,8 +584,8 @@ int64_t dsw_rmsnorm_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype) {
 int dsw_rmsnorm_bwd(const void* G, const void* D, const void* X, int64_t ldx, const void* R, int64_t ldr, const void* W, const float* rstd, void* dX, void* dW,
                     void* workspace, int64_t workspace_bytes, int64_t rows, int64_t C, int dtype, dsw_stream_t stream) {
     if (!dtype_ok(dtype)) return DSW_ERR_BAD_DTYPE;
-    if (!rows_ok(rows, C) || ldx < C || (R && ldr < C) || !W || (!dX && !dW)) return DSW_ERR_BAD_ARG;
-    if (rows > 0 && (!G || !X || !rstd)) return DSW_ERR_BAD_ARG;
+    if (!rows_ok(rows, C) || ldx < C || (R && ldr < C) || !W) return DSW_ERR_BAD_ARG;
+    if (rows > 0 && (!G || !X || !rstd || (!dX && !dW))) return DSW_ERR_BAD_ARG;       // (without rows dX is an empty tensor's null)
     if (dW && (!workspace || workspace_bytes < dsw_rmsnorm_bwd_workspace_bytes(rows, C, dtype))) return DSW_ERR_WORKSPACE;
     if (rows == 0 && !dW) return DSW_OK;
     hipStream_t s = (hipStream_t)stream;
