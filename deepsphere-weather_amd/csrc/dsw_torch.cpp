@@ -333,7 +333,8 @@ Tensor dense_mix_fp8(const Tensor& xq, const Tensor& xs, const Tensor& wq, const
     on_gpu(xq);
     const c10::DeviceGuard guard(xq.device());
     constexpr int64_t far = 1 << 23;                   // rows further apart are copied (the tiles use 32-bit offsets)
-    const Tensor w = (k > 1 && wq.stride(1) != 1) || wq.stride(0) < k || wq.stride(0) >= far ? wq.contiguous() : wq;
+    const bool w_rows = (k == 1 || wq.stride(1) == 1) && (n == 1 || (wq.stride(0) >= k && wq.stride(0) < far));
+    const Tensor w = w_rows ? wq : wq.contiguous();
     Rows x = as_rows(xq);
     if (x.step >= far) x = as_rows(xq.contiguous());
     const Rows s = as_rows(xs, true);
@@ -341,7 +342,7 @@ Tensor dense_mix_fp8(const Tensor& xq, const Tensor& xs, const Tensor& wq, const
     std::vector<int64_t> sizes(xq.sizes().begin(), xq.sizes().end());
     sizes.back() = n;
     const Tensor y = at::empty(sizes, xq.options().dtype(dtype));
-    const int64_t w_step = std::max(w.stride(0), k);
+    const int64_t w_step = n == 1 ? k : w.stride(0);
     const auto low = [](const void* p) { return (int64_t)(reinterpret_cast<uintptr_t>(p) & 15); };
     const bool aligned = (low(x.t.data_ptr()) | low(w.data_ptr()) | ((x.step | w_step | k) & 15)) == 0;
     const int64_t bytes = lib.fp8_mix_workspace_bytes(x.rows, n, k, aligned);
