@@ -10,13 +10,13 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 
 #include <array>
 #include <cmath>
-#include <functional>
 #include <optional>
 #include <string>
 #include <vector>
@@ -73,7 +73,8 @@ void on_gpu(const Tensor& t) {
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 // (a result without a tangent would read as a derivative of zero; no_grad does not switch tangents off)
-void no_tangent(std::initializer_list<const Tensor*> tensors) {
+void no_tangent(at::ArrayRef<const Tensor*> tensors) {
+    if (!torch::autograd::ForwardADLevel::try_get_by_idx(0)) return;       // (no tensor of the process has a tangent)
     for (const Tensor* t : tensors)
         TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "dsw: the row norm, the 8-bit channel mix and the gradient norm have no "
                     "forward-mode derivative; unpack the dual tensor (torch.autograd.forward_ad.unpack_dual)");
@@ -379,11 +380,14 @@ Tensor grad_norm_clip(std::vector<Tensor> grads, const std::optional<std::vector
             TORCH_CHECK_VALUE(dense(to[i]), "dsw: a clipped tensor must be dense (cover consecutive elements, in any dimension order)");
         }
     }
-    for (const auto& list : {std::cref(grads), std::cref(to)})
-        for (const Tensor& t : list.get()) {
-            no_tangent({&t});
-            TORCH_CHECK(!at::GradMode::is_enabled() || !wants_grad(t), "dsw: the gradient norm and the clipping have no backward pass; call them under torch.no_grad() or detach() the tensors");
-        }
+    std::vector<const Tensor*> all;
+    all.reserve(2 * n);
+    for (const Tensor& t : grads) all.push_back(&t);
+    if (clip && out) for (const Tensor& t : to) all.push_back(&t);
+    no_tangent(all);
+    if (at::GradMode::is_enabled())
+        for (const Tensor* t : all)
+            TORCH_CHECK(!wants_grad(*t), "dsw: the gradient norm and the clipping have no backward pass; call them under torch.no_grad() or detach() the tensors");
     on_gpu(grads[0]);
     const c10::DeviceGuard guard(dev);
     const at::AutoGradMode off(false);
