@@ -3,7 +3,7 @@
 // 128-byte dgrad-plane rows.  This program moves exactly those bytes with no arithmetic to speak of, in the two
 // traversal orders a kernel can choose (each workgroup a contiguous slab of rows / tiles interleaved across the grid),
 // so that the kernel's achieved bandwidth can be set against what the memory system gives THIS access pattern rather
-// than against a two-stream copy.   hipcc --offload-arch=gfx950 -O3 tools/stream_mix.hip -o /tmp/stream_mix && /tmp/stream_mix
+// than against a two-stream copy.   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/stream_mix.hip -o /tmp/stream_mix && /tmp/stream_mix
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>
