@@ -4,9 +4,11 @@
 // bf16 output: one 16x16x128 8-bit matrix instruction covers a whole scale block: its result is multiplied by the block's scale and
 // added to the running fp32 sum, so no scale is ever applied to an 8-bit value.  Inside the instruction the products of 8
 // neighbouring k are aligned to the largest exponent among them and cut 13 bits below it (measured with sums of two products;
-// groups of 8 are joined in fp32): a relative 1.5e-5 of a random block, two orders below half a step of bf16.
+// groups of 8 are joined in fp32): a relative 1.5e-5 of a random block, two orders below half a step of bf16.  That is relative to
+// the products, not to their sum: where large ones cancel, what is left can be smaller than the loss (fp32 output is for those).
 // fp32 output: the cut would show, so the e4m3 values are widened to bf16 (exact) and multiplied by bf16 instructions (exact
 // products, fp32 sums, 1e-8 of a random block), at half the matrix rate.
+// The two scales of a block are multiplied first, in fp32, and their product scales the block's sum.
 // The WEIGHT rows are the instruction's row operand and the activation rows its column operand: a lane then holds four
 // neighbouring outputs n of ONE activation row m, needs one scale per block, and stores neighbouring outputs.
 // (Which k a byte of the operand registers stands for does not matter as long as both operands agree on it.)

@@ -7,7 +7,7 @@
 // share the row, and everything that a pass can derive from the row leaves in the same pass.  The square sum and the norm use
 // the unrounded fp32 sum x + r; h itself is rounded to the storage type once.  The backward pass takes the two addends rather than
 // the rounded h: with bf16 storage the rounding would be as large an error in dw as dw's own (1.5 x together); the price is
-// a fifth stream, 50 MB of 250 at 98304 x 256.
+// a fifth stream, 50 MB of 250 at 98304 x 256, and that both addends stay alive until then.
 #include "dsw_rows_common.h"
 #include "../../include/dsw_hip.h"
 
@@ -428,8 +428,12 @@ static int launch_fwd(const NormArgs& a, hipStream_t s) {
     return DSW_ERR_BAD_ARG;
 }
 
-// workgroups of the backward pass (= rows of `part`): two per CU, each with the next row in flight (98304 x 256 bf16: 47.4 us =
-// 5.3 TB/s; 768: 48.6, 1024: 52.9; without the next row ahead 52.5 at 1024 and 78.7 at 512.  8192 x 4096: 69.4, 74.7, 79.8)
+// workgroups of the backward pass (= rows of `part`): two per CU with each group's next row in flight, as many as fit where a thread
+// holds up to two vectors (98304 x 256 bf16: 768: 48.6, 1024: 52.9, against 47.4; without the next row ahead 52.5 at 1024 and 78.7
+// at 512.  8192 x 4096: 69.4, 74.7, 79.8).  Four vectors (279-292 registers) leave room for one workgroup per CU at a time, which costs
+// little; eight in bf16 spill.  2^25 elements each, us of this kernel and its five (fp32: four) streams in TB/s:
+//   bf16, 256: 64 (5.2)   1024: 61 (5.5)   2048: 65 (5.1)   4096: 64 (5.2)   6144: 82 (4.1)   8192: 73 (4.6)   12288: 215 (1.6)
+//   fp32, 256: 111 (4.8)  2048: 109 (4.9)  4096: 115 (4.7)  8192: 115 (4.7)
 constexpr int RN_BWD_BLOCKS = 512;
 static long bwd_blocks(int64_t rows, int64_t C, int dtype) {
     const int V = dtype == DSW_BF16 ? 8 : 4;

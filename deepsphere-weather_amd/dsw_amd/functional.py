@@ -1283,8 +1283,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.
 
 def rms_norm_residual(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6):
     """``(rms_norm(h), h)`` with ``h = x + residual``, in one pass: ``h`` is the stream that the next residual addition
-    takes, the norm is taken of the unrounded sum.  Backward returns ONE tensor as the gradient of both addends.  A backward
-    pass that is captured into a graph while an earlier graph over the same leaf lives on another stream is refused."""
+    takes, the norm is taken of the unrounded sum.  Backward returns ONE tensor as the gradient of both addends; with bf16 it
+    reads both again (``h`` is their rounded sum, which would show in the weight's gradient), so they stay alive until then, one
+    tensor more than ``h`` alone.  A backward pass that is captured into a graph while an earlier graph over the same leaf lives on another stream is refused."""
     return _native.ops().rms_norm_residual(x, residual, weight, eps)
 
 
@@ -1309,7 +1310,8 @@ def quantize_fp8_weight(weight: torch.Tensor) -> Fp8Weight:
 def dense_mix_fp8(x, weight: Fp8Weight, bias: torch.Tensor = None, dtype: torch.dtype = None) -> torch.Tensor:
     """``y = x @ weight (+ bias)`` over the last axis on the 8-bit matrix cores: every block of 128 channels is summed in fp32,
     scaled by its two scales and added in fp32 (a bf16 output uses 8-bit matrix instructions, which drop what lies 13 bits below
-    the largest of 8 neighbouring products; an fp32 output exact products).  ``x``: :class:`Fp8Rows`, or an fp32 / bf16 tensor
+    the largest of 8 neighbouring products - where large products cancel, ask for an fp32 output: exact products).  The two scales of
+    a block are multiplied first, in fp32.  ``x``: :class:`Fp8Rows`, or an fp32 / bf16 tensor
     (quantised first); ``dtype``: the output's (default: the tensor's, bfloat16 for rows), which ``bias [Fout]`` shares.  Serving
     only (no backward)."""
     if not isinstance(weight, Fp8Weight):

@@ -436,8 +436,8 @@ def get_conv_fun(conv_type):
 
 class RMSNorm(torch.nn.Module):
     """Root-mean-square norm over the channels of every node of ``(sample, node, channel)`` tensors, an extension next to the
-    reference's ``BatchNorm1d`` option: it needs neither batch statistics (an autoregressive rollout has one sample) nor the two
-    transposes, and takes the residual's addition with it.
+    reference's ``BatchNorm1d`` option: a node's own channels are its statistics (none are kept between training and rollout, none
+    mix samples), there are no transposes, and it takes the residual's addition with it.
 
     ``norm(x)`` -> y;  ``norm(x, residual)`` -> ``(y, x + residual)``;  ``norm.rows_fp8(x, residual)`` -> the same with y as
     8-bit rows for :func:`dsw_amd.functional.dense_mix_fp8` (serving, under ``torch.no_grad()``)."""

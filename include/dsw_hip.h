@@ -434,7 +434,7 @@ int dsw_quant_fp8_weight(const void* W, int64_t stride_in, int64_t stride_out, v
  * stored H may stand for the sum: X = H, R = NULL, at the price of its rounding in dW), rstd as stored:
  *     dX = D + rstd (G w - xhat mean_c(G w xhat)),  xhat = h rstd     (the gradient of x AND of r);     dW = sum_rows G xhat
  * dX or dW may be NULL.  G, D, dX dense.  The workspace (dsw_rmsnorm_bwd_workspace_bytes) is needed for dW; no atomics: equal
- * inputs give equal bits.  rows == 0: dW = 0. */
+ * inputs give equal bits.  rows == 0: dW = 0 (dX and dW may then both be NULL). */
 int64_t dsw_rmsnorm_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype);
 int dsw_rmsnorm_bwd(const void* G, const void* D, const void* X, int64_t ldx, const void* R, int64_t ldr, const void* W, const float* rstd, void* dX, void* dW,
                     void* workspace, int64_t workspace_bytes, int64_t rows, int64_t C, int dtype, dsw_stream_t stream);
@@ -445,7 +445,9 @@ int dsw_rmsnorm_bwd(const void* G, const void* D, const void* X, int64_t ldx, co
  * Any K, N >= 1 and alignments; rows that are not 16-byte aligned or no multiple of 16 bytes long (aligned = 0; bases, strides and K
  * of both operands) are copied into the workspace first when there are more than 64 of them.  The order of every sum is fixed by the sizes.  fp32 output: exact products, fp32 sums.  bf16
  * output: the 8-bit matrix instructions, which within 8 neighbouring k drop what lies 13 bits below the largest product, then sum
- * in fp32: each group of 8 loses at most 7 * 2^-13 of its largest product (relative 2-norm of random rows: 1.5e-5). */
+ * in fp32: each group of 8 loses at most 7 * 2^-13 of its largest product (relative 2-norm of random rows: 1.5e-5; where large
+ * products cancel that is no bound relative to Y).  XS * WS of a block is formed first, in fp32: it must not overflow, and one below
+ * 2^-126 loses bits. */
 int64_t dsw_fp8_mix_workspace_bytes(int64_t M, int64_t N, int64_t K, int aligned);
 int dsw_fp8_mix(const void* X, int64_t ldx, const float* XS, int64_t xs_row, int64_t xs_blk, const void* W, int64_t ldw,
                 const float* WS, const void* bias, void* Y, int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
