@@ -99,7 +99,7 @@ class _NodeLinear(Linear):
         super().__init__(*args, **kwargs)
         self._lay_out_weight()
 
-    _serving = None      # (the weight (weakly), its version) while the 8-bit path is on
+    _serving = None      # (the weight (weakly; None: not one tensor), its version) while the 8-bit path is on
 
     def serve_fp8(self, enable=True):
         """Inference through the 8-bit channel mix (weight: a scale per 128 x 128 block, rows: a scale per 128 channels).  Only
@@ -109,20 +109,23 @@ class _NodeLinear(Linear):
         captured one too, quantises the weight's present values (512 -> 128 channels: 5 us), and nothing of it is kept."""
         self._serving = None
         if enable:
+            weight = self.weight
             with torch.no_grad():
-                dsw_functional.quantize_fp8_weight(self.weight.t())     # (what cannot be served raises here)
-            self._serving = (weakref.ref(self.weight), self.weight._version)
+                dsw_functional.quantize_fp8_weight(weight.t())     # (what cannot be served raises here)
+            # (a parametrised weight is another tensor each time it is asked for)
+            self._serving = (weakref.ref(weight) if self.weight is weight else None, weight._version)
         return self
+
+    def _quantized(self):
+        made_from, version = self._serving
+        if (made_from is not None and made_from() is not self.weight) or self.weight._version != version:
+            raise RuntimeError("the weight has changed since serve_fp8(): call it again (or serve_fp8(False))")
+        return dsw_functional.quantize_fp8_weight(self.weight.t())
 
     @property
     def _fp8(self):
         """``(Fp8Weight,)`` of the weight's present values while the 8-bit path is on, else None."""
-        if self._serving is None:
-            return None
-        weight, version = self._serving
-        if weight() is not self.weight or self.weight._version != version:
-            raise RuntimeError("the weight has changed since serve_fp8(): call it again (or serve_fp8(False))")
-        return (dsw_functional.quantize_fp8_weight(self.weight.t()),)
+        return None if self._serving is None else (self._quantized(),)
 
     def serves_fp8(self):
         """Whether a call now takes the 8-bit path."""
@@ -150,7 +153,7 @@ class _NodeLinear(Linear):
 
     def forward(self, x):
         if self.serves_fp8():
-            return dsw_functional.dense_mix_fp8(x, self._fp8[0], self.bias)
+            return dsw_functional.dense_mix_fp8(x, self._quantized(), self.bias)
         # `weight.t()` is dense [in, out] for the column-major parameter; a row-major tensor (SWAG sample, user
         # assignment) is made contiguous inside dense_mix - same values either way
         # (the parameter's gradient buffer, if a GradBucket in direct mode attached one: memory order [in][out], which is

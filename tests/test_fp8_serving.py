@@ -5,6 +5,7 @@ import io
 
 import pytest
 import torch
+import torch.nn.utils.parametrize  # noqa: F401
 
 from dsw_amd import functional as F
 from modules import my_models_graph as M
@@ -68,6 +69,21 @@ def test_states_that_are_assigned(stand_ins):
         assert _right(lin, x)
         lin.serve_fp8()
         assert _served(lin, x) is not None and _right(lin, x)
+
+
+def test_a_parametrised_weight(stand_ins):
+    """Its layer has another tensor each time it is asked for the weight: what is served follows the parameters below it."""
+    class Twice(torch.nn.Module):
+        def forward(self, w):
+            return 2 * w
+
+    x = torch.randn(5, 6)
+    lin = M._NodeLinear(6, 4)
+    torch.nn.utils.parametrize.register_parametrization(lin, "weight", Twice())
+    lin.serve_fp8()
+    for _ in range(2):
+        assert _served(lin, x) is not None and _right(lin, x)
+        lin.parametrizations.weight.original.data.add_(1.0)
 
 
 def test_copies_start_in_their_own_precision(stand_ins):
