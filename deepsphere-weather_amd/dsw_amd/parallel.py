@@ -343,6 +343,7 @@ class GradBucket:
 
     __call__ = finish
 
+    @torch.no_grad()
     def clip_norm(self, max_norm, norm_type=2.0):
         """Scale the gradients by ``min(1, max_norm / (norm + 1e-6))`` with the norm (1, 2 or inf) of all of them taken together,
         and return that norm (0-dim, on the device).  Call it after ``finish()``: the averaged gradients are the same on every

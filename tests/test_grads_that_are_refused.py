@@ -43,6 +43,12 @@ def test_clipping_a_bucket_does_not_mind_parameters():
         lin(torch.randn(2, 4)).sum().backward()
         with passed():
             bucket.clip_norm(1.0)
+    for p in lin.parameters():                        # gradients with a graph of their own are clipped as torch clips them: under no_grad
+        p.grad = None
+    lin(torch.randn(2, 4)).square().sum().backward(create_graph=True)
+    assert lin.weight.grad.requires_grad
+    with passed():
+        bucket.clip_norm(1.0)
 
 
 def test_forward_mode_derivatives_are_refused():
