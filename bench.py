@@ -5,13 +5,13 @@
 
 One "step" = one forward + backward pass of the hot path over one batch of synthetic HEALPix
 fields already resident in HBM (plus, for N > 1, the single flat-bucket RCCL all-reduce of the
-parameter gradients).  Metric (BASELINE.json): HEALPix nodes*channels/sec through ConvCheb (fwd+bwd)
+parameter gradients).  Metric: HEALPix nodes*channels/sec through ConvCheb (fwd+bwd)
 = B * V * Fin * n_gpus / t_step.  Scaling is weak: every rank owns a full per-GPU batch.
 
 Workloads
-  ns    north-star shape: nside=64 (V=49152), K=3, 32->64 channels, B=16 per GPU, fp32   (default)
-  c3    BASELINE configs[2]: nside=64, K=5, 64->128, B=16 per GPU, bf16 storage / fp32 accumulate
-  unet  BASELINE configs[1]: UNetSpherical nside=32, K=3, B=8 per GPU, fp32, interp pooling
+  ns    default shape: nside=64 (V=49152), K=3, 32->64 channels, B=16 per GPU, fp32   (default)
+  c3    nside=64, K=5, 64->128, B=16 per GPU, bf16 storage / fp32 accumulate
+  unet  UNetSpherical nside=32, K=3, B=8 per GPU, fp32, interp pooling
 
 Launch.  `python bench.py --gpus N` with N > 1 and no torchrun environment starts the N ranks itself (it re-executes
 under `python -m torch.distributed.run --nnodes=1 --nproc-per-node N --master-addr 127.0.0.1`, one process per GPU,
@@ -48,7 +48,7 @@ WORKLOADS = {
     "ns": dict(nside=64, K=3, fin=32, fout=64, batch=16, dtype="f32"),
     "c3": dict(nside=64, K=5, fin=64, fout=128, batch=16, dtype="bf16"),
     "unet": dict(nside=32, K=3, fin=18, fout=2, batch=8, dtype="f32"),
-    # BASELINE configs[4]: equiangular 200 x 400 (V = 80 000, irregular degree at the poles), k = 20, K = 3, 32 ch,
+    # equiangular 200 x 400 (V = 80 000, irregular degree at the poles), k = 20, K = 3, 32 ch,
     # interpolation pooling to the HEALPix nside=32 sampling and back (pooling BETWEEN samplings)
     "c5": dict(nside=0, nlat=200, nlon=400, K=3, fin=32, fout=32, batch=8, dtype="f32"),
 }
@@ -159,7 +159,7 @@ def make_unet(wl, knn, device):
 
 
 def spmm_algorithmic_bytes(E, Lb, K):
-    """forward recurrence [2 + 3(K-2)] E + (K-1) Lb, adjoint [3 + 4(K-2)] E + (K-1) Lb."""
+    """Bytes by definition: forward recurrence [2 + 3(K-2)] E + (K-1) Lb, adjoint [3 + 4(K-2)] E + (K-1) Lb."""
     fwd = (2 + 3 * (K - 2)) * E + (K - 1) * Lb
     bwd = (3 + 4 * (K - 2)) * E + (K - 1) * Lb
     return fwd, bwd
@@ -356,7 +356,7 @@ def graph_kernel_durations(seq, n_steps=40, timeout=150):
 def roofline_leg(layer, x, steps, warmup, traffic_key=None, pmc_leg=None, traced=None, ms_per_step=None):
     """The SpMM recurrence launches of the workload's dominant ConvCheb layer against the HBM roofline.  Durations of
     everything a timed step launches come from `traced` (trace_steps: in-step HIP events); launches the step does NOT make
-    (the forward recurrence alone at the north-star shape, the stand-alone channel mix) are timed as isolated legs and
+    (the forward recurrence alone at the default shape, the stand-alone channel mix) are timed as isolated legs and
     say so."""
     from dsw_amd import functional as F_
 
@@ -459,11 +459,11 @@ def roofline_leg(layer, x, steps, warmup, traffic_key=None, pmc_leg=None, traced
     t_gemm = tr("bwd_gemm_fused", V, C, Fout)
     t_dgrad, t_wgrad = tr("bwd_dgrad", V, C, Fout), tr("bwd_wgrad", V, C, Fout)
     t_adj = tr("basis_adj", V, C, K)
-    t_bwdf = None                                      # (the mix-first one-launch dX was retired in round 6)
+    t_bwdf = None                                      # (the mix-first one-launch dX is retired)
     t_dual = tr("bwd_dual", V, C, Fout)                # whole backward in one launch in the dual form (dsw_bwd3d.hip)
     have_trace = t_adj is not None or t_bwdf is not None or t_dual is not None or mf
 
-    # forward recurrence alone: in the step where the step launches it, otherwise an isolated leg (north-star gate)
+    # forward recurrence alone: in the step where the step launches it, otherwise an isolated leg (forward-recurrence gate)
     fwd_s_iso = timed(fwd)
     fwd_s = t_bfwd["avg_us"] * 1e-6 if (fwd_rec_in_step and t_bfwd is not None and t_h2m is None) else fwd_s_iso
     adj_s_iso = None
@@ -477,14 +477,14 @@ def roofline_leg(layer, x, steps, warmup, traffic_key=None, pmc_leg=None, traced
 
     yb_bytes = N * Fout * es
     mm_peak = MFMA_PEAK_TFLOPS["bf16" if x.dtype == torch.bfloat16 else "f32"]
-    mix_flops = 2.0 * N * C * K * Fout          # one contraction over (k, f): forward mix, dgrad or wgrad (SURVEY 8d)
+    mix_flops = 2.0 * N * C * K * Fout          # one contraction over (k, f): forward mix, dgrad or wgrad
     hop1_b = spmm_algorithmic_bytes(E, Lb, 2)[0]
 
-    # ---- one entry per role the step launches.  SURVEY 8(d) splits a ConvCheb layer's work in two: the SpMM recurrence is
+    # ---- one entry per role the step launches.  The byte count splits a ConvCheb layer's work in two: the SpMM recurrence is
     # priced in BYTES against HBM (`bytes_8d`: [2 + 3 (K - 2)] E + (K - 1) Lb forward, [3 + 4 (K - 2)] E + (K - 1) Lb adjoint),
     # the channel-mix contractions in FLOPS against the matrix peak of the storage dtype.  A fused launch carries both: its
     # recurrence bytes over its in-graph time is `hbm_frac`, its flops over the same time `mfma_frac` - GEMM operand bytes of
-    # an unfused design are never added to the byte count (VERDICT r5: no entry can exceed 1 by construction of the count).
+    # an unfused design are never added to the byte count (no entry can exceed 1 by construction of the count).
     # `frac` repeats the fraction of the entry's `bound`.
     def entry(role, kernel, t, bound, rec_b=None, flops=None, compulsory=None, leg=None, gemm_bytes=None, n_launch=None):
         # `us` = everything the role launches per call (a fused launch + its small reduce; the K - 1 hops of a recurrence);
@@ -556,7 +556,7 @@ def roofline_leg(layer, x, steps, warmup, traffic_key=None, pmc_leg=None, traced
     for d in in_step:
         d["share"] = round(d["us"] * d["calls"] / max(step_sum_us, 1e-9), 3)
 
-    # ---- headline: the DOMINANT launch among those that carry SpMM recurrence work in the step (SURVEY 8d bytes of its
+    # ---- headline: the DOMINANT launch among those that carry SpMM recurrence work in the step (recurrence bytes of its
     # recurrence / its in-graph duration); the whole step's recurrence bytes over the whole step's time beside it
     rec = [d for d in in_step if "bytes_8d" in d]
     if rec:
@@ -596,14 +596,14 @@ def roofline_leg(layer, x, steps, warmup, traffic_key=None, pmc_leg=None, traced
         out["step_frac"] = round(rec_bytes_step / (ms_per_step * 1e-3) / 1e9 / HBM_PEAK_GBS, 4)
         out["step_flops"] = flops_step
         out["step_mfma_frac"] = round(flops_step / (ms_per_step * 1e-3) / 1e12 / mm_peak, 4)
-    # second launch of the step by time, flat (the driver's parser keeps scalars of this object only)
+    # second launch of the step by time, flat (scalars only: a short parser keeps those)
     others = sorted((d for d in in_step if d is not dom), key=lambda d: -d["us"] * d["calls"])
     if others:
         o = others[0]
         out.update({"second_kernel": o["kernel"], "second_us": o["us"], "second_bound": o["bound"], "second_frac": o["frac"],
                     "second_hbm_frac": o.get("hbm_frac"), "second_mfma_frac": o.get("mfma_frac"),
                     "second_frac_counter": o.get("frac_counter")})
-    # north-star gate: the K = 3 forward recurrence alone (in the step where the step launches it, else an isolated leg)
+    # forward-recurrence gate: the K = 3 forward recurrence alone (in the step where the step launches it, else an isolated leg)
     out.update({"fwd_recurrence_us": round(fwd_s * 1e6, 2), "fwd_recurrence_frac": round(fwd_b / fwd_s / 1e9 / HBM_PEAK_GBS, 4),
                 "fwd_recurrence_in_step": bool(fwd_rec_in_step and t_bfwd is not None and t_h2m is None),
                 "forward_path": path_names.get(fwd_path),
@@ -643,7 +643,7 @@ def roofline_leg(layer, x, steps, warmup, traffic_key=None, pmc_leg=None, traced
 def pooling_leg(model, run_forward, steps, traffic_key=None, pmc_leg=None, traced=None):
     """The interpolation-pooling products of the workload (RemapBlock: pool / unpool and their transposed backward), each
     with its own shape: bytes = input rows + output rows + operator (int32 column + fp32 value per entry + row pointers),
-    time = HIP events around `steps` back-to-back calls.  north_star names this kernel; the U-Net has 4 distinct products
+    time = HIP events around `steps` back-to-back calls.  The U-Net has 4 distinct products
     (x2 directions), workload c5 the cross-sampling pair."""
     from dsw_amd import functional as F_
     from modules.layers import RemapBlock
@@ -1324,11 +1324,11 @@ def main():
             dist.destroy_process_group()
         return
     probe = timed_region(args.steps)
-    # The contract times exactly K steps; K steps of this workload are a ~10 ms region at the driver's K = 20, short
+    # The contract times exactly K steps; K steps of this workload are a ~10 ms region at K = 20, short
     # enough for a single clock-ramp or scheduling hiccup to move the number by 10-20 %.  So the region is repeated
     # back to back - every repetition is exactly K steps inside its own barrier + synchronize bracket - until >= 1.5 s
     # (--min-timed-ms) have been timed, and the MEDIAN region is reported (all regions are summarised in "region_ms").
-    # (1.5 s also keeps the GPU visibly busy for a sampling monitor; round 2's 150 ms fell between its samples.)
+    # (1.5 s also keeps the GPU visibly busy for a sampling monitor; 150 ms fell between its samples.)
     n_regions = int(min(1000, max(3, -(-(args.min_timed_ms * 1e-3) // max(probe, 1e-6)))))
     regions = sorted(timed_region(args.steps) for _ in range(n_regions))
     elapsed = regions[len(regions) // 2]
@@ -1356,7 +1356,7 @@ def main():
             "batch_per_gpu": B, "global_batch": args.global_batch if args.global_batch is not None else B * world, "nodes": V,
             "parallelism": "dp%d (batch shards, flat-bucket %s grad all-reduce)" % (
                 world, "RCCL" if not dist.is_initialized() or dist.get_backend() == "nccl" else dist.get_backend()),
-            # N = 1 and N > 1 do not run byte-identical steps (ADVICE r3): say which one this line timed
+            # N = 1 and N > 1 do not run byte-identical steps: say which one this line timed
             "grad_handling": ("parameter gradients live in one flat bucket (one memset per step), the weight-gradient kernels "
                               "add into it, all-reduced in place" if bucket.active() else
                               "parameter gradients live in one flat bucket (one memset per step), the weight-gradient kernels "
@@ -1405,7 +1405,7 @@ def main():
         out["grad_sync"] = {"max_abs_diff_across_ranks": diff, "identical": diff == 0.0,
                             "grad_l2": float(mine.double().norm())}
     if rank == 0 and world == 1:
-        # SURVEY 8(d): per-iteration HIP-event times (outside the timed region above): median and p10 / p90
+        # per-iteration HIP-event times (outside the timed region above): median and p10 / p90
         n_ev = 100
         evs = [(torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)) for _ in range(n_ev)]
         for a, b in evs:
@@ -1470,7 +1470,7 @@ def main():
                 out["roofline"].update({"pooling_us_per_step": po["us_per_step"], "pooling_frac": po["frac"],
                                         "pooling_frac_counter": po["frac_counter"]})
             # the long form (every role of the step, the pooling products, the stand-alone recurrence / GEMM legs) goes to a side
-            # file - the line itself stays short enough for the driver to keep whole - or inline on request
+            # file - the line itself stays short enough to be kept whole - or inline on request
             if args.detail == "inline":
                 out["roofline"]["detail"] = detail
             elif args.detail != "none":

@@ -102,7 +102,7 @@ static inline int64_t w_image_bytes(int64_t Fin, int64_t Fout, int64_t K, int dt
     if (zdg > m) m = zdg;
     const int64_t copy = Fin * K * Fout * 4;
     // + the scratch of the streaming GEMM's balanced decomposition (dsw_gemm_x3s.hip: 4 KiB of flags, one partial 256 x 128
-    // fp32 tile per workgroup, 256 workgroups) - only for layers one of whose GEMMs can take that kernel (ADVICE r4: the
+    // fp32 tile per workgroup, 256 workgroups) - only for layers one of whose GEMMs can take that kernel (the
     // 32-channel layers paid 32 MiB of scratch per backward call for a kernel they never launch)
     const bool streams = dtype == DSW_F32 && (w_may_stream(K * Fin, Fout) || w_may_stream(Fout, K * Fin) ||
                                                w_may_stream(Fin, K * Fout) || w_may_stream(K * Fout, Fin));

@@ -578,7 +578,7 @@ int dsw_cheb3_bwd_dual_eligible(const dsw_hop2_plan* plan_t, int64_t V, int64_t 
     static const char* env = dsw_diag_env("DSW_BWD_DUAL");   // "0": separate dgrad / wgrad / adjoint launches (diagnostics / A-B)
     if (env && env[0] == '0') return 0;
     if (dtype != DSW_F32 || K != 3 || Fin != 32 || (Fout != 64 && Fout != 32)) return 0;
-#ifdef DSW_D3_NO_FOUT32      // A/B builds: 32 -> 32 layers on the route over the basis planes, as before round 6
+#ifdef DSW_D3_NO_FOUT32      // A/B builds: 32 -> 32 layers on the route over the basis planes, as before
     if (Fout == 32) return 0;
 #endif
     if (!plan_t || plan_t->hops == 1 || plan_t->tile_rows != 64 || plan_t->explicit_tiles || !dsw_spmm2_supported(plan_t, Fin, dtype)) return 0;

@@ -51,7 +51,7 @@ static inline const char* dsw_diag_env(const char*) { return nullptr; }
 
 // Build flags of this translation unit, collected at load time (dsw_build_flags()): a library any of whose objects was
 // compiled with a diagnostics / ablation switch is refused by dsw_amd._native.load() unless it was asked for by path
-// (DSW_HIP_LIB) - a variant build is one -D away from a wrong-by-design product library (VERDICT r4).
+// (DSW_HIP_LIB) - a variant build is one -D away from a wrong-by-design product library.
 #define DSW_FLAG_DIAG 1
 #define DSW_FLAG_ABLATION 2
 #if defined(DSW_DIAG)
@@ -63,7 +63,7 @@ static inline const char* dsw_diag_env(const char*) { return nullptr; }
     defined(DSW_ABL_F3_NOSPLIT) || defined(DSW_F3_PLAIN_STORE) || defined(DSW_ABL_F3_NOLOAD) || defined(DSW_ABL_F3_NOSTORE) || defined(DSW_ABL_F3_NOMFMA) || defined(DSW_ABL_B3_NOSPLIT) || \
     defined(DSW_ABL_B3_NOGATHER) || defined(DSW_ABL_B3_NOMFMA) || defined(DSW_STAGE_EARLY) || defined(DSW_ABL_B3_NOLOAD) || defined(DSW_ABL_B3_NOFRAG) || \
     defined(DSW_GATHER_N) || defined(DSW_F3_YBOUNCE) || defined(DSW_F3_SKEW) || defined(DSW_D3_SKEW) || defined(DSW_D3_WG_PER_CU) || \
-    defined(DSW_D3_NO_FOUT32) || defined(DSW_X3S_NO_DIRECT) || defined(DSW_X3S_BFRAG_ALL) || defined(DSW_ABL_X3S_NOB) || defined(DSW_X3S_LB4) || defined(DSW_X3S_FORCE_NT2)   /* round-6 A/B switches (correct results, other schedules) */
+    defined(DSW_D3_NO_FOUT32) || defined(DSW_X3S_NO_DIRECT) || defined(DSW_X3S_BFRAG_ALL) || defined(DSW_ABL_X3S_NOB) || defined(DSW_X3S_LB4) || defined(DSW_X3S_FORCE_NT2)   /* A/B switches (correct results, other schedules) */
 #define DSW_TU_F_ABL DSW_FLAG_ABLATION
 #else
 #define DSW_TU_F_ABL 0

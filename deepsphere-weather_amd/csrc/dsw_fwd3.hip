@@ -16,7 +16,7 @@
 //   * the "B" operand are the tile rows.  Every row is split ONCE, by the thread that produces it (the staging thread
 //     for X, the phase-1 / phase-2 thread for T1 / T2: 5.5 VALU per element), into three bf16 images in LDS
 //     ([plane][term][64 rows][64 B], 36 KB), from which each wave reads ready-made fragments (one ds_read_b128 per
-//     term).  What this replaces, measured at the north-star shape: splitting on the fly in every wave that shares a
+//     term).  What this replaces, measured at the default shape: splitting on the fly in every wave that shares a
 //     row (4 column blocks): +32 M VALU instructions, 181 us; v_mfma_f32_16x16x4_f32 (no split): 165 us - the fp32
 //     MFMA issues at the VECTOR rate and did not overlap with the other workgroup's gather FMAs (removing the MFMAs
 //     gave back 47 of its 61 us);

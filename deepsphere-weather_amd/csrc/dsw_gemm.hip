@@ -275,7 +275,7 @@ __global__ __launch_bounds__(256) void ts_gemm_kernel(const TsGemmParams P) {
 // wgrad: partial[s][(k*Fin + f)][o] = sum_{n in slab s} T_k[n, f] * dY[n, o]; row Kd = column sums
 // ---------------------------------------------------------------------------------------------
 // NW waves per workgroup = number of 32-row (k, f) tiles it covers (1..4): no idle waves when
-// K * ceil(Fin/32) is not a multiple of 4 (north-star: 3 tiles -> 3-wave workgroups).
+// K * ceil(Fin/32) is not a multiple of 4 (default layer: 3 tiles -> 3-wave workgroups).
 // ALIGNED: Fin % 32 == 0, Fout-tile full and 16-byte aligned rows (no column bounds checks).
 template <bool BF16, int NW, bool ALIGNED>
 __global__ __launch_bounds__(64 * NW) void cheb_wgrad_kernel(const WgradParams P) {

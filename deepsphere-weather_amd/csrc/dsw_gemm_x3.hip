@@ -6,7 +6,7 @@ using namespace dsw_gemm;
 namespace {
 // STREAM variants (IO bit 3): the A operand is larger than half of the 256 MB Infinity Cache - its rows are read with
 // nontemporal loads (they cannot stay resident anyway, and streaming them past the caches leaves those to the W panel
-// and to what the neighbouring kernels exchange).  Same-box: C3 -1.8 %, C5 -1.7 %, k = 20 north-star -2.3 %; the UNet's
+// and to what the neighbouring kernels exchange).  Same-box: C3 -1.8 %, C5 -1.7 %, k = 20 of the 32 -> 64 layer -2.3 %; the UNet's
 // layers (A <= 75 MB, re-read by up to three column tiles out of L2) keep cached loads (+0.3 % with nontemporal ones).
 template <bool NT>
 static __device__ __forceinline__ f32x4 lda16(const void* p) {

@@ -7,7 +7,7 @@
 // Workgroup = NWV waves, tile = (32 * NWV rows) x (32 * NT columns); a wave owns 32 rows and NT MFMA tiles.
 // Per 32-wide reduction chunk:
 //   A: 3-deep register prefetch ring -> the wave's private staging rows in LDS (no workgroup barrier), split
-//      into bf16 terms in registers right before the MFMAs (as in the resident kernel); round 6, 8-wave form with the
+//      into bf16 terms in registers right before the MFMAs (as in the resident kernel); 8-wave form with the
 //      pre-split W image (DIRECT): the ring IS the operand - a lane loads its 2 x 8 values of the MFMA layout, no LDS;
 //   B: the chunk's [32 k][32 * NT cols] fp32 block of W is fetched one chunk ahead into registers, split ONCE per
 //      workgroup into three bf16 planes and written to LDS as [plane][col][k] (k contiguous, 80-byte rows ->
@@ -437,7 +437,7 @@ __global__ __launch_bounds__(64 * NWV, DSW_X3S_WAVES_PER_EU(PRE, NWV)) void ts_g
                     }
                 // RELEASE: every wave drains ITS OWN stores before the barrier (the compiler emits only vmcnt(63) here - the
                 // stores are fire-and-forget for it - and a gfx950 workgroup barrier does not wait for memory operations), so
-                // the flag below cannot become visible before any byte of the piece (ADVICE r4, high)
+                // the flag below cannot become visible before any byte of the piece
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 __syncthreads();
                 if (tid == 0) __hip_atomic_store(P.sk_flags + slot0 + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);

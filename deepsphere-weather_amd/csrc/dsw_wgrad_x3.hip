@@ -64,8 +64,8 @@ static __device__ __forceinline__ void split_store(unsigned short* dst, const in
         const float m0 = trunc_bf16(r0), m1 = trunc_bf16(r1), m2 = trunc_bf16(r2), m3 = trunc_bf16(r3);
         *reinterpret_cast<u32x2*>(dst + plane_elems) = pack4(m0, m1, m2, m3);
         *reinterpret_cast<u32x2*>(dst + 2 * plane_elems) = pack4(r0 - m0, r1 - m1, r2 - m2, r3 - m3);
-        // (the residuals as register pairs - v_pk_add_f32, half the subtractions - measured +-0 on the NS step and the U-Net
-        // in round 4: the split is not what this loop waits for)
+        // (the residuals as register pairs - v_pk_add_f32, half the subtractions - were +-0 on the NS step and the
+        // U-Net: the split is not what this loop waits for)
     }
 }
 
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(64 * NW, FUSE ? 2 : 1) void cheb_wgrad_x3_kernel(co
     constexpr int PF = FUSE ? 2 : 3;                    // the fused variant needs the registers of the third slot
     constexpr int TPLANE = BLK;                         // one (wave, plane) T tile
     // dY image: NO blocks [32 n][32 o] per plane, 64-byte rows.  Two things keep BOTH ways it is read off the bank
-    // conflicts the plain layout had (41 % of the LDS-active cycles at the north-star shape, PMC round 2):
+    // conflicts the plain layout had (41 % of the LDS-active cycles at the default shape, by counters):
     //  * the 16-byte chunks of a row are XOR-swizzled with (n >> 2) & 3: the fused dgrad reads the image by ROWS (lane =
     //    row, 16 bytes at a fixed column), and rows n, n + 4, n + 8, n + 12 of a 64-byte-row image share their banks -
     //    a 4-way conflict on every read; with the swizzle the 16 rows of a read phase hit 16 distinct bank quads.  The
@@ -671,7 +671,7 @@ int dsw_wgrad_x3_try_launch(WgradParams& P, int bf16, int64_t max_slabs, int64_t
 
 // wgrad with the dgrad of the same rows fused in (fp32, aligned, plain basis-first backward).  Applies when one
 // workgroup sees all of Fout (64 or 128 columns) and all (k, f) tiles (<= 4 waves) and the W^T panel keeps two
-// workgroups per CU: the small layers of the path (north-star shape 32 -> 64, K = 3).  Returns 1 when it took the launch.
+// workgroups per CU: the small layers of the path (default shape, 32 -> 64, K = 3).  Returns 1 when it took the launch.
 int dsw_wgrad_dgrad_fused_try_launch(WgradParams& P, int bf16, int64_t max_slabs, int64_t* S_out, hipStream_t stream,
                                      int* rc) {
     static const char* x3env = dsw_diag_env("DSW_GEMM_X3");

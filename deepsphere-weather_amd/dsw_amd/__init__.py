@@ -2,7 +2,7 @@
 
 Chebyshev graph convolution (ConvCheb / conv_cheb) and sparse interpolation pooling
 (RemapBlock) behind the reference's own nn.Module API; see ``modules/`` next to this package for
-the drop-in import path (``modules.layers`` etc.) and DESIGN.md at the repo root.
+the drop-in import path (``modules.layers`` etc.).
 """
 from . import _native  # noqa: F401
 from .functional import (  # noqa: F401

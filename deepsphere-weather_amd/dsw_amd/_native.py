@@ -145,7 +145,7 @@ def load():
     flags = int(lib.dsw_build_flags())
     if flags and not os.environ.get("DSW_HIP_LIB"):
         # a diagnostics build (environment overrides of the kernel selection) or an ablation build (kernels with phases cut
-        # out: wrong results by design) must never stand in for the product library by accident (VERDICT r4)
+        # out: wrong results by design) must never stand in for the product library by accident
         raise DswNativeError(
             f"{LIB_PATH} is a diagnostics build (dsw_build_flags() = {flags}: bit 0 DSW_DIAG, bit 1 ablation switches); "
             "rebuild the product library (`python -m dsw_amd.build --force`) or name the variant explicitly with DSW_HIP_LIB")

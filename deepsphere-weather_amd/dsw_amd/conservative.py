@@ -3,7 +3,7 @@
 The reference obtains its pooling / unpooling matrices from ``xsphere.compute_interpolation_weights(method=
 "conservative", normalization="fracarea")`` (``/root/reference/modules/layers.py:531-581``): xsphere builds the
 spherical Voronoi mesh of each sampling's nodes and lets the CDO binary (``gencon``) integrate the overlap areas of the
-cells.  Neither xsphere nor CDO is available (SURVEY.md 8c), so this module restates the published algorithm:
+cells.  Neither xsphere nor CDO is available, so this module restates the published algorithm:
 
 1. cells = spherical Voronoi regions of the node positions (``scipy.spatial.SphericalVoronoi``) - convex geodesic
    polygons;

@@ -354,7 +354,7 @@ def _aligned16(t):
     """A backward without basis planes (``T`` = None) exists only as the one-launch dual form, whose 16-byte vector loads need
     16-byte aligned operands.  Tensors torch allocates are (256-byte) aligned; a contiguous VIEW into a flat buffer at an odd
     element offset (flattened parameter / gradient buckets of other frameworks) is not: it is copied once - rare, and cheaper
-    than keeping the planes for everybody (ADVICE r5: the shape check of the forward cannot see the backward's pointers)."""
+    than keeping the planes for everybody (the shape check of the forward cannot see the backward's pointers)."""
     return t if t is None or t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
@@ -428,7 +428,7 @@ class _HipBackend:
         that backward runs in the dual form (``dsw_cheb_bwd_needs_basis`` == 0: X and dY only) AND the forward is the
         one-launch kernel, the basis planes are neither allocated nor stored and ``T`` comes back as None.
         ``no_backward=True`` (inference, ``torch.no_grad()``): no backward will ever run, so the planes are dropped wherever
-        the forward can do without them, without building the plan of the transposed operator (ADVICE r5)."""
+        the forward can do without them, without building the plan of the transposed operator."""
         lib = _native.load()
         B, V, Fin = x.shape
         _, K, Fout = w.shape
@@ -473,7 +473,7 @@ class _HipBackend:
     @staticmethod
     def _bwd_workspace(lib, x, Fin, Fout, K, dt):
         """Scratch of one backward call.  The size depends on the CU count of the CURRENT device (slabs of the one-launch dual
-        backward): queried under the guard of the tensor's device, where the launch will run (ADVICE r5)."""
+        backward): queried under the guard of the tensor's device, where the launch will run."""
         with torch.cuda.device(x.device):
             nbytes = int(lib.dsw_cheb_bwd_workspace_bytes(x.shape[0], x.shape[1], Fin, Fout, K, dt))
         if nbytes < 0:
@@ -570,7 +570,7 @@ class _HipBackend:
     # handle inherits the previous stream's workspace, which is sound: the kernel re-arms the ticket at the end of every call,
     # so a workspace is only ever left half-armed by an aborted kernel (a device fault ends the process).  The cache is
     # BOUNDED (least recently used entry dropped beyond _RPG_WS_MAX; torch's stream pool has 32 streams per device), so
-    # short-lived streams cannot leak workspaces without limit (ADVICE r4).
+    # short-lived streams cannot leak workspaces without limit.
     _rpg_ws = {}
     _RPG_WS_MAX = 64
 
@@ -720,7 +720,7 @@ def _padded_width(fin: int, dtype) -> int:
     """Input width the kernels should see.  The fast paths (whole-forward kernel, two-hop pairs, bf16-pipe GEMMs, fused
     backward pass) want rows of whole 32-channel chunks; a layer with, say, 18 input channels (the U-Net's first:
     3 time steps x 6 fields) otherwise takes the exact-fp32 kernels with predicated scalar loads - 4 launches, 150 us =
-    4 % of the U-Net step (round 2).  Zero channels contribute exact zeros, so such a layer is evaluated as the next
+    4 % of the U-Net step.  Zero channels contribute exact zeros, so such a layer is evaluated as the next
     multiple of 32 (x and the weight rows padded with zeros, the gradients sliced back) whenever that is at most twice
     the real width: 16..31 -> 32, 33..63 -> 64, ...  fp32 only (the bf16 paths have other alignment rules)."""
     if not PAD_INPUT_CHANNELS or dtype != torch.float32 or fin % 32 == 0:

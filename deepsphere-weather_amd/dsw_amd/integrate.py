@@ -11,7 +11,7 @@ Two explicit, side-effect-visible helpers instead:
 
 ``load_reference_modules(root, names)``
     loads the REFERENCE's own files for the given submodules (default: its model definitions) under the ``modules.*``
-    names, on top of THIS package's ``modules.layers`` - the call-compatibility setup of SURVEY.md 8(a8)/(b): the
+    names, on top of THIS package's ``modules.layers`` - the call-compatibility setup: the
     reference's ``UNetSpherical`` then runs unchanged on the HIP kernels.
 """
 from __future__ import annotations

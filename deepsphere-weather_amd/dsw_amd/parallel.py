@@ -5,7 +5,7 @@ weights are replicated), so forward and backward need no collective.  The only e
 all-reduce of the parameter gradients per step.  The payload is tiny (24.8 KB for a 32->64 K=3
 layer, 7.08 MB for the whole UNetSpherical), i.e. latency-bound on the fully connected 7-link xGMI
 topology: everything goes in a single flat bucket so RCCL runs one collective, not one per tensor.
-The reference itself has no multi-GPU path (SURVEY.md section 2).
+The reference itself has no multi-GPU path.
 """
 from __future__ import annotations
 
@@ -198,7 +198,7 @@ class GradBucket:
         self._direct = False
         self._dirty = False       # a backward ran inside no_sync(): the hooks did not count, finish() sends everything
         # a bucket built earlier on the same parameters may have left its direct-accumulation pointers behind: the
-        # kernels would keep adding into THAT buffer while p.grad is a view of this one (ADVICE r3)
+        # kernels would keep adding into THAT buffer while p.grad is a view of this one
         for p in self.params:
             if hasattr(p, "_dsw_grad_acc"):
                 del p._dsw_grad_acc

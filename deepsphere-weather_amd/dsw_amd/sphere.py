@@ -245,7 +245,7 @@ def gauss_legendre_vec(nlat: int, nlon="ecmwf-octahedral"):
 # equivariance): they scale with the pixel size, ~ c_k / nside; c_k below are the nside = 32 values times 32.  pygsp's
 # sphere-graphs branch keeps the full per-(k, nside) table (`_OPTIMAL_KERNEL_WIDTHS`), which is not vendored with the
 # reference: these figures are quoted from the paper, the 1 / nside scaling is an approximation (the table's own entries
-# drift from it by ~2 %) - parity with pygsp's graphs stays UNPINNED (DESIGN.md, section 4).
+# drift from it by ~2 %) - parity with pygsp's graphs stays UNPINNED.
 HEALPIX_KERNEL_WIDTH_TIMES_NSIDE = {8: 0.02500 * 32, 20: 0.03185 * 32, 40: 0.042432 * 32, 60: 0.051720 * 32}
 
 
@@ -253,7 +253,7 @@ def knn_graph_laplacian(coords: np.ndarray, k: int, lap_type: str = "normalized"
     """Symmetrised k-NN Gaussian graph and its Laplacian (scipy CSR, float64).
 
     Weight ``exp(-d^2 / (2 s^2))``.  ``kernel_width``: ``None`` - ``s^2`` = the mean SQUARED k-NN distance (this
-    module's rule since round 1); ``"mean"`` - ``s`` = the mean k-NN distance (the default rule of pygsp's ``NNGraph``);
+    module's rule from the start); ``"mean"`` - ``s`` = the mean k-NN distance (the default rule of pygsp's ``NNGraph``);
     a float - that width (e.g. ``healpix_kernel_width``).  Symmetrisation keeps an edge if either endpoint selected it
     (so degrees are >= k and irregular where the sampling is anisotropic, e.g. equiangular poles).
     """

@@ -25,7 +25,7 @@ this file                      reference ``modules/layers.py``
 
 The arithmetic (``torch.sparse.mm`` at ``:164,167,962`` and ``matmul`` at ``:177`` plus the layout
 copies around them) is replaced by ``dsw_amd.functional`` -> ``libdsw_hip.so``.  Everything that is
-not on that path (image convolutions, HEALPix/equiangular max/avg pooling, cotan Laplacian) is out of scope and raises ``NotImplementedError`` with a pointer to DESIGN.md.
+not on that path (image convolutions, HEALPix/equiangular max/avg pooling, cotan Laplacian) is out of scope and raises ``NotImplementedError``.
 """
 import math
 from abc import ABC, abstractmethod
@@ -39,7 +39,7 @@ from dsw_amd import functional as _F
 
 _OUT_OF_SCOPE = (
     "{} is outside the ConvCheb / interpolation-pooling hot path rebuilt for MI355X "
-    "(see DESIGN.md, 'Out of scope'); use the reference implementation for it."
+    "(out of scope); use the reference implementation for it."
 )
 
 _RELU_LIKE = {
@@ -250,7 +250,7 @@ def build_pooling_matrices(src_graph, dst_graph):
     The reference derives them from CDO conservative-remap weights via ``xsphere``
     (``layers.py:531-581``).  When that tool-chain is importable it is used; otherwise the
     self-contained builder of ``dsw_amd.sphere`` supplies matrices with the same invariants
-    (row-stochastic pool / unpool) - value parity with CDO is unpinned, see DESIGN.md.
+    (row-stochastic pool / unpool) - value parity with CDO is unpinned.
     """
     try:
         from xsphere.remapping import compute_interpolation_weights  # noqa: F401

@@ -190,7 +190,7 @@ class ResBlock(torch.nn.Module):
             torch.nn.init.constant_(last.bn.weight, 0)
             torch.nn.init.constant_(last.bn.bias, 0)
 
-    # Block-level fusion (SURVEY 8 f1, VERDICT r2 item 6) is IMPLEMENTED and OFF: measured same-box on the U-Net workload
+    # Block-level fusion is IMPLEMENTED and OFF: measured same-box on the U-Net workload
     # (nside 32, B 8: 3.93 ms plain) every variant was slower - backward only (ReZero scale inside the dgrad kernels,
     # dscale = <W, dW_raw> + <b, db_raw>) +0.4 %, + forward epilogue +0.9 %, + fork +0.8 %, everything +1.8 %: the
     # passes they remove run out of the Infinity Cache at these sizes (50 MB tensors), while a residual operand in the

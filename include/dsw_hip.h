@@ -76,7 +76,7 @@ typedef struct dsw_hop2_plan {
     int64_t struct_bytes;      /* sizeof(dsw_hop2_plan) of the header the CALLER was built with (since 0.1.1).  Every entry point
                                   that takes a plan refuses one of another size (DSW_ERR_BAD_ARG; the *_supported predicates
                                   say 0): the struct grew between versions, and a caller built against an older header would
-                                  otherwise have the library read past the end of its struct (ADVICE r5). */
+                                  otherwise have the library read past the end of its struct. */
 } dsw_hop2_plan;
 
 /* Library version (major*10000 + minor*100 + patch). */
@@ -95,7 +95,7 @@ int dsw_build_flags(void);
  * the kernel's completion signal, what a profiler's kernel trace reports - no marker packets between the kernels), and the
  * entry points note on the host which role the kernels belong to.  A benchmark opens a trace, runs steps the ordinary way
  * (eagerly: nothing is recorded inside a stream capture) and reads the roles back - every kernel timed INSIDE the step, with
- * the caches in the state the step leaves them, which back-to-back calls of one kernel are not (VERDICT r4: isolated timings
+ * the caches in the state the step leaves them, which back-to-back calls of one kernel are not (isolated timings
  * were 11-14 % off the in-step durations).  One trace at a time, process-wide.
  *   dsw_trace_begin(capacity)  room for `capacity` kernel launches; starts recording.
  *   dsw_trace_end(...)         waits for the recorded kernels and writes up to `cap` KERNEL records in launch order: index of
@@ -120,7 +120,7 @@ int dsw_build_flags(void);
 #define DSW_ROLE_ZMIX 11           /* mix-first forward: plane GEMM Z_k = X W_k */
 #define DSW_ROLE_CLENSHAW_FWD 12   /* mix-first forward: Clenshaw recurrence on the output channels */
 #define DSW_ROLE_ELEMENTWISE 13    /* relu mask (kind 1), ReZero residual forward (2) / backward (3), ReZero parameter gradients (4) */
-#define DSW_ROLE_BWD_FUSED 14      /* (retired in round 6 with dsw_cheb_dx_one_launch: never emitted) */
+#define DSW_ROLE_BWD_FUSED 14      /* (retired with dsw_cheb_dx_one_launch: never emitted) */
 #define DSW_ROLE_FWD_HOP2_MIX 16     /* hop 2 + channel mix + bias of the forward in one launch (one-hop plans) */
 #define DSW_ROLE_BASIS_DUAL 15     /* mix-first backward: Chebyshev basis of dY under L^T (on the output channels) */
 #define DSW_ROLE_RMSNORM 18          /* row norm (aux: rows, C, 0 forward / 1 forward with 8-bit output / 4 backward), 8-bit rows (2), 8-bit weights (3) */
@@ -199,7 +199,7 @@ int dsw_spmm2_supported(const dsw_hop2_plan* plan, int64_t C, int dtype);
  * U, Z, Z2, Y: [B, V, C]; Z / Z2 may be NULL; Y may alias Z or Z2 (a tile reads them on its own rows only), not U.
  * The form the recurrences take on DENSE stencils (the reference's default k = 20 graph, utils_config.py:50: 21-23
  * entries per row), where the first-hop redundancy of the fused pair costs more than the round trip of the
- * intermediate plane it saves (DESIGN.md section 3).  stream_out = 1: nontemporal stores (nothing gathers Y next).
+ * intermediate plane it saves.  stream_out = 1: nontemporal stores (nothing gathers Y next).
  * Returns DSW_ERR_BAD_ARG if dsw_spmm_staged_supported() is 0. */
 int dsw_spmm_staged(const dsw_hop2_plan* plan, int64_t V, const void* U, const void* Z, const void* Z2, void* Y,
                     int64_t B, int64_t C, float a, float b, float c, int dtype, dsw_stream_t stream, int stream_out);
@@ -313,7 +313,7 @@ int dsw_cheb_fwd_ws(const int32_t* rowptr, const int32_t* colind, const float* v
 int dsw_relu_bwd(const void* dY, const void* Y, void* dYm, int64_t n, int dtype, dsw_stream_t stream);
 
 /* 0 if dsw_cheb_bwd of this layer shape works WITHOUT the forward's basis planes (T = NULL): mix-first layers, K = 1, and
- * layers whose whole backward runs in one launch in the dual form (dsw_bwd3d.hip: fp32, K = 3, 32 -> 64 or - round 6 -
+ * layers whose whole backward runs in one launch in the dual form (dsw_bwd3d.hip: fp32, K = 3, 32 -> 64 or
  * 32 -> 32, two-hop plan of L^T, V % 64 == 0):
  *     U_k = T_k(L^T) dY on chip,   dX = sum_k U_k W_k^T,   dW_k = X^T U_k,   db = 1^T dY
  * - X and dY in, dX out, no T_1 / T_2 and no dgrad planes.  The forward of such a layer may then be called with T = NULL

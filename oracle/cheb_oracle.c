@@ -4,7 +4,7 @@
  * numpy fp64 closed form in cheb_oracle.py): scalar loops, double accumulation, no dependencies.
  * Follows /root/reference/modules/layers.py:113-180 (conv_cheb: T0 = x, T1 = L x, Tk = 2 L T(k-1) - T(k-2),
  * y = [T0|..|T(K-1)] W with W indexed [f][k][o]), :375 (bias) and :956-964 (RemapBlock), in the node-major
- * [B, V, C] layout.  Backward is the hand-derived adjoint (SURVEY.md 8a1), valid for non-symmetric L.
+ * [B, V, C] layout.  Backward is the hand-derived adjoint, valid for non-symmetric L.
  * Checked against the golden fixtures recorded from the reference (tests/test_oracle_golden.py).
  * Only tests / smoke / the bench cpu_baseline leg may load it; the product never does.
  *

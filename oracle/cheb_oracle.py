@@ -5,7 +5,7 @@ the product.  Only ``tests/``, ``__graft_entry__.smoke()`` and ``bench.py``'s
 ``cpu_baseline`` leg may import it.  The shipped path (``deepsphere-weather_amd/``) never
 does and raises if its HIP library is missing.
 
-Pinning: the reference has no tests / golden vectors of its own (SURVEY.md section 4), so
+Pinning: the reference has no tests / golden vectors of its own, so
 this oracle is pinned against outputs of the reference itself, imported in the build
 container by ``tests/golden/make_golden.py`` and committed as ``tests/golden/*.npz``
 (``tests/test_oracle_golden.py`` checks every fixture).
@@ -17,7 +17,7 @@ Two independent restatements are kept:
   ATen CPU kernels.  This is the ``cpu_baseline`` ("port") that ``bench.py`` times.
 * ``cheb_forward_f64`` / ``cheb_backward_f64`` - closed form in the native ``[B, V, C]``
   layout, float64 numpy + scipy CSR, with the hand-derived backward
-  (SURVEY.md section 8a1), independent of autograd.
+  independent of autograd.
 """
 from __future__ import annotations
 
@@ -227,7 +227,7 @@ def _to_f64(a):
 
 
 def max_rel_err(a, ref):
-    """max |a - ref| / max |ref|  (the normalisation used for the tolerances in SURVEY 8c)."""
+    """max |a - ref| / max |ref|  (the normalisation used for the tolerances)."""
     a = _to_f64(a)
     ref = _to_f64(ref)
     denom = np.max(np.abs(ref))

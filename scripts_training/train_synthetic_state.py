@@ -19,7 +19,7 @@ estimate is not deterministic, so independently built replicas would not share o
     python scripts_training/train_synthetic_state.py --config_file configs/UNetSpherical/Healpix_400km/InterpPool-Graph_knn.synthetic.json --steps 20
     python -m torch.distributed.run --nnodes=1 --nproc-per-node 8 --master-addr 127.0.0.1 scripts_training/train_synthetic_state.py ...
 
-The AR schedule of xforecasting itself is external to the reference repository (parity unpinned, DESIGN.md 4).
+The AR schedule of xforecasting itself is external to the reference repository (parity unpinned).
 """
 import argparse
 import inspect
@@ -57,7 +57,7 @@ def synthetic_tensor_info(cfg):
     ms, syn, ar = cfg["model_settings"], cfg["synthetic_settings"], cfg["ar_settings"]
     sampling = ms["sampling"].lower()
     if sampling != "healpix":
-        raise NotImplementedError("the synthetic driver builds HEALPix samplings (DESIGN.md section 7)")
+        raise NotImplementedError("the synthetic driver builds HEALPix samplings")
     n_node = 12 * int(ms["sampling_kwargs"]["subdivisions"]) ** 2
     n_in = syn["n_dynamic_features"] + syn["n_bc_features"]
     return {
@@ -199,7 +199,7 @@ class Trainer:
             self.graph = None
             torch.cuda.synchronize()
             # a capture that died inside finish() leaves chunks marked as launched and works of the aborted recording
-            # behind: the first eager backward would raise "a second backward()..." 
+            # behind: the first eager backward would raise "a second backward()..."
             self.bucket.reset()
         if self.distributed:
             # ALL ranks replay the graph or NONE does: a rank that fell back issues its chunk all-reduces in hook order,

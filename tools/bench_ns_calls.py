@@ -1,5 +1,5 @@
 #!/usr/bin/env python3
-"""The three calls of the north-star step (dsw_cheb_fwd, the backward GEMM pass + adjoint = dsw_cheb_bwd), each replayed from
+"""The three calls of the default step (dsw_cheb_fwd, the backward GEMM pass + adjoint = dsw_cheb_bwd), each replayed from
 its own HIP graph of 20 calls and from one graph of the whole step: us per call.  For A/B runs of experiment builds:
     DSW_HIP_LIB=_ab_libs/x.so python tools/bench_ns_calls.py [knn]"""
 import os, sys

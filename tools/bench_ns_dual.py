@@ -1,5 +1,5 @@
 #!/usr/bin/env python3
-"""The one-launch dual backward (dsw_bwd3d.hip) of the north-star layer: parity against the plan-less route of dsw_cheb_bwd
+"""The one-launch dual backward (dsw_bwd3d.hip) of the default layer: parity against the plan-less route of dsw_cheb_bwd
 (dgrad GEMM + plain adjoint hops + wgrad from the forward's basis planes) and against an fp64 closed form, then us per call
 of both full backwards and of the forward with / without basis stores, replayed from HIP graphs.
     python tools/bench_ns_dual.py [nside] [B]"""

@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """One configuration of the K = 3 recurrences for profiling (tools/pmc_pair.sh):
     tools/bench_pair_one.py <unused 0|1> <knn> [fwd|adj] [nside C B]
-(the first argument selected the row-group kernel of the round-3 experiment, branch exp/quad-gather; ignored on main)"""
+(the first argument selected the row-group kernel of an earlier experiment; ignored)"""
 import os, sys
 REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path[:0] = [os.path.join(REPO, "deepsphere-weather_amd"), REPO]

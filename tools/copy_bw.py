@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
 """Calibration: achievable HBM streaming rates on this box (torch copy / add kernels) for the
-tensor sizes of the north-star workload.  Prints GB/s counting bytes read + written."""
+tensor sizes of the default workload.  Prints GB/s counting bytes read + written."""
 import torch
 
 dev = "cuda:0"

@@ -1,4 +1,4 @@
-// Practical HBM ceiling for the STREAM MIX of the fused backward GEMM pass of the north-star layer (dsw_wgrad_x3.hip,
+// Practical HBM ceiling for the STREAM MIX of the fused backward GEMM pass of the default layer (dsw_wgrad_x3.hip,
 // FUSE): per row of N = B*V it reads three 128-byte basis rows (T0..T2) and one 256-byte dY row and writes three
 // 128-byte dgrad-plane rows.  This program moves exactly those bytes with no arithmetic to speak of, in the two
 // traversal orders a kernel can choose (each workgroup a contiguous slab of rows / tiles interleaved across the grid),
@@ -80,7 +80,7 @@ static float run(const f4* T0, const f4* T1, const f4* T2, const f4* dY, f4* G0,
 }
 
 int main() {
-    const long n_rows = 16L * 49152;            // the north-star batch: B = 16 spheres of nside 64
+    const long n_rows = 16L * 49152;            // the default batch: B = 16 spheres of nside 64
     const size_t row32 = 32 * sizeof(float);
     f4 *T0, *T1, *T2, *dY, *G0, *G1, *G2;
     CK(hipMalloc(&T0, n_rows * row32)); CK(hipMalloc(&T1, n_rows * row32)); CK(hipMalloc(&T2, n_rows * row32));
