@@ -79,8 +79,8 @@ def test_a_rung_that_fails_is_the_ranks_failure(tmp_path, body, code):
 
 
 def test_a_rung_that_cannot_end_itself_is_killed(tmp_path):
-    """No guard of its own: the supervisor's limit (its run limit and a minute: 15 s here) ends it."""
-    p = _start(tmp_path, "time.sleep(600) if attempt == 0 else bench.print_line({'metric': 'm'})", DSW_BENCH_TIMEOUT="-50")
+    """No guard of its own: the supervisor's limit (its run limit and a minute: 24 s here) ends it."""
+    p = _start(tmp_path, "time.sleep(600) if attempt == 0 else bench.print_line({'metric': 'm'})", DSW_BENCH_TIMEOUT="-40")
     out, err = p.communicate(timeout=120)
     assert p.returncode == 0 and out.splitlines() == ['{"metric": "m"}'], err[-1500:]
     assert [r[1:3] for r in _log(tmp_path)] == [["0", "0"], ["1", "0"]]
